@@ -10,7 +10,8 @@ Two layers:
   ``nvfp4_swizzle_scales``, ``nvfp4_gemm``, ``w4a16_gemm``, ``fp4_gemv`` -- device pointers as torch tensors;
 * tensor-level helpers used by the tests and the benchmark: ``quantize``, ``amax``, ``gemm``, ``linear``, the MoE
   layer (``moe_route``, ``moe_forward`` with its chained and fused-norm forms, ``moe_layer`` with the router fused
-  in, ``MoeExperts``), and the
+  in, ``MoeExperts``), the MXFP4 operators (``mx_quantize``, ``mx_geglu_quantize``, ``mx_dequantize``, ``mx_gemm``),
+  and the
   expert-parallel entry points (``ep_*`` over NCCL slots, ``ep_p2p_*`` over peer memory with the ``ipc_*`` set-up
   helpers; ``expert_parallel.py`` orchestrates them).
 """
@@ -231,6 +232,170 @@ def hbm_read_stream(buf: torch.Tensor, rows: int, row_bytes: int) -> None:
     if buf.numel() * buf.element_size() < rows * row_bytes:
         raise ValueError("hbm_read_stream: buffer smaller than rows * row_bytes")
     _check("hbm_read_stream", lib().nvfp4b_hbm_read_stream(buf.data_ptr(), rows, row_bytes, _stream()))
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# MXFP4 (include/nvfp4_b200.h: nvfp4b_mx_*)
+# ----------------------------------------------------------------------------------------------------------------
+# These check what they are given before anything is launched (ValueError), run on the tensors' device whatever the
+# current one is, and allocate outputs that are not given on the stream that the call runs on.
+
+def _mx_sigs():
+    L = lib()
+    if getattr(L, "_mx_ready", False):
+        return L
+    ll = ctypes.c_longlong
+    sig = {
+        "nvfp4b_mx_scale_buffer_bytes": ([ctypes.c_int, ctypes.c_int], ctypes.c_size_t),
+        "nvfp4b_mx_swizzle_scales": ([_P, _P, ctypes.c_int, ctypes.c_int, _P], ctypes.c_int),
+        "nvfp4b_mx_quantize_bf16": ([_P, ll, ctypes.c_int, ctypes.c_int, _P, _P, _P], ctypes.c_int),
+        "nvfp4b_mx_quantize_f32": ([_P, ll, ctypes.c_int, ctypes.c_int, _P, _P, _P], ctypes.c_int),
+        "nvfp4b_mx_geglu_quantize": ([_P, ll, ctypes.c_int, ctypes.c_int, _P, _P, _P], ctypes.c_int),
+        "nvfp4b_mx_dequantize": ([_P, _P, ctypes.c_int, ctypes.c_int, _P, ctypes.c_int, ll, _P], ctypes.c_int),
+        "nvfp4b_mx_gemm": ([_P, _P, _P, _P, ctypes.c_float, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P,
+                            ctypes.c_int, ll, _P], ctypes.c_int),
+    }
+    for name, (args, res) in sig.items():
+        f = getattr(L, name)
+        f.argtypes = args
+        f.restype = res
+    L._mx_ready = True
+    return L
+
+
+def _rows(name: str, t: torch.Tensor, dtypes, shape, device=None) -> int:
+    """Checks a [rows, columns] CUDA tensor with unit column stride; returns its row pitch in elements.  None in
+    `shape` stands for any size."""
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: dtype {t.dtype}, expected one of {dtypes}")
+    if t.dim() != 2 or any(w is not None and w != g for w, g in zip(shape, t.shape)):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise ValueError(f"{name}: on {t.device}, expected {device or 'a CUDA device'}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: columns must be contiguous")
+    pitch = t.stride(0) if rows > 1 else max(cols, 1)
+    if pitch < cols:
+        raise ValueError(f"{name}: rows overlap (row stride {pitch})")
+    return pitch
+
+
+def _flat(name: str, t: torch.Tensor, dtype, numel: int, device) -> None:
+    """Checks a contiguous tensor of at least `numel` elements."""
+    if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < numel:
+        raise ValueError(f"{name}: needs {numel} contiguous {dtype} elements on {device}, got {t.numel()} of {t.dtype} "
+                         f"on {t.device}")
+
+
+def _empty(shape, dtype, device, stream) -> torch.Tensor:
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _launch(name: str, fn, device, stream, *args) -> None:
+    """fn(*args, stream) with `device` current; `stream` None = that device's current stream."""
+    if isinstance(stream, torch.cuda.Stream) and stream.device != device:
+        raise ValueError(f"{name}: stream on {stream.device}, tensors on {device}")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _check(name, fn(*args, _stream(stream)))
+    _check(name, fn(*args, _stream(stream)))
+
+
+def mx_scale_buffer_bytes(outer: int, K: int) -> int:
+    """Bytes of the tile-layout e8m0 scales of an MXFP4 [outer, K] operand."""
+    return -(-outer // 128) * -(-K // 128) * 512 if outer > 0 and K > 0 else 0
+
+
+def mx_swizzle_scales(logical: torch.Tensor, outer: int, K: int, stream=None) -> torch.Tensor:
+    """Logical e8m0 scales [outer, K/32] uint8 (as a checkpoint holds them) -> tile layout."""
+    _flat("mx_swizzle_scales: logical", logical, torch.uint8, outer * (K // 32), logical.device)
+    out = _empty(mx_scale_buffer_bytes(outer, K), torch.uint8, logical.device, stream)
+    _launch("mx_swizzle_scales", _mx_sigs().nvfp4b_mx_swizzle_scales, logical.device, stream, _ptr(logical),
+            _ptr(out), outer, K)
+    return out
+
+
+def _mx_buffers(name, M, K, codes, scales, device, stream):
+    if K % 32:
+        raise ValueError(f"{name}: width {K} is not a multiple of 32")
+    if codes is None:
+        codes = _empty((M, K // 2), torch.uint8, device, stream)
+    else:
+        _flat(f"{name}: codes", codes, torch.uint8, M * (K // 2), device)
+    if scales is None:
+        scales = _empty(mx_scale_buffer_bytes(M, K), torch.uint8, device, stream)
+    else:
+        _flat(f"{name}: scales", scales, torch.uint8, mx_scale_buffer_bytes(M, K), device)
+    return codes, scales
+
+
+def mx_quantize(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None, stream=None):
+    """MXFP4-quantise a bf16 or fp32 [M, K] device tensor (K % 32 == 0; rows may be strided, with a row pitch of a
+    multiple of 16 bytes).  Returns (codes [M, K/2] uint8, tile-layout e8m0 scales uint8)."""
+    ld = _rows("mx_quantize: x", x, (torch.bfloat16, torch.float32), (None, None))
+    M, K = x.shape
+    codes, scales = _mx_buffers("mx_quantize", M, K, codes, scales, x.device, stream)
+    L = _mx_sigs()
+    fn = L.nvfp4b_mx_quantize_bf16 if x.dtype == torch.bfloat16 else L.nvfp4b_mx_quantize_f32
+    _launch("mx_quantize", fn, x.device, stream, _ptr(x), ld, M, K, _ptr(codes), _ptr(scales))
+    return codes, scales
+
+
+def mx_geglu_quantize(gate_up: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+                      stream=None):
+    """gelu_tanh(gate) * up of bf16 rows [gate (I) | up (I)], quantised to MXFP4 (the codes of the float64 value).
+    Returns (codes [M, I/2] uint8, tile-layout e8m0 scales uint8), the second product's A operand."""
+    ld = _rows("mx_geglu_quantize: gate_up", gate_up, (torch.bfloat16,), (None, None))
+    M, I = gate_up.shape[0], gate_up.shape[1] // 2
+    if gate_up.shape[1] % 2:
+        raise ValueError("mx_geglu_quantize: odd width")
+    codes, scales = _mx_buffers("mx_geglu_quantize", M, I, codes, scales, gate_up.device, stream)
+    _launch("mx_geglu_quantize", _mx_sigs().nvfp4b_mx_geglu_quantize, gate_up.device, stream, _ptr(gate_up), ld, M, I,
+            _ptr(codes), _ptr(scales))
+    return codes, scales
+
+
+def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
+                  out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """The values of MXFP4 codes [M, K/2] and tile-layout scales as bf16 or fp32 [M, K] (exact in both)."""
+    _rows("mx_dequantize: codes", codes, (torch.uint8,), (None, None))
+    M, K = codes.shape[0], 2 * codes.shape[1]
+    _mx_buffers("mx_dequantize", M, K, codes, scales, codes.device, stream)
+    if out is None:
+        out = _empty((M, K), dtype, codes.device, stream)
+    ld = _rows("mx_dequantize: out", out, (torch.bfloat16, torch.float32), (M, K), codes.device)
+    _launch("mx_dequantize", _mx_sigs().nvfp4b_mx_dequantize, codes.device, stream, _ptr(codes), _ptr(scales), M, K,
+            _ptr(out), 1 if out.dtype == torch.float32 else 0, ld)
+    return out
+
+
+def mx_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
+            out: torch.Tensor | None = None, out_kind: int = OUT_BF16_ROWMAJOR, alpha: float = 1.0,
+            stream=None) -> torch.Tensor:
+    """D = alpha * A @ B^T on the MXFP4 tensor cores.  A: codes [M, K/2]; B: codes [N, K/2]; tile-layout scales.  D is
+    [M, N] bf16 or fp32 (rows may be strided), or fp32 [N, M] with OUT_F32_COLMAJOR, as in ``gemm``."""
+    _rows("mx_gemm: a", a, (torch.uint8,), (None, None))
+    M, half = a.shape
+    _rows("mx_gemm: b", b, (torch.uint8,), (None, half), a.device)
+    N, K, dev = b.shape[0], 2 * half, a.device
+    _mx_buffers("mx_gemm: a", M, K, a, a_scales, dev, stream)
+    _mx_buffers("mx_gemm: b", N, K, b, b_scales, dev, stream)
+    if out_kind not in (OUT_BF16_ROWMAJOR, OUT_F32_COLMAJOR, OUT_F32_ROWMAJOR):
+        raise ValueError(f"mx_gemm: unknown out_kind {out_kind}")
+    shape = (N, M) if out_kind == OUT_F32_COLMAJOR else (M, N)
+    dtype = torch.bfloat16 if out_kind == OUT_BF16_ROWMAJOR else torch.float32
+    if out is None:
+        out = _empty(shape, dtype, dev, stream)
+    ldd = _rows("mx_gemm: out", out, (dtype,), shape, dev)
+    _launch("mx_gemm", _mx_sigs().nvfp4b_mx_gemm, dev, stream, _ptr(a), _ptr(a_scales), _ptr(b), _ptr(b_scales),
+            float(alpha), M, N, K, _ptr(out), out_kind, ldd)
+    return out
 
 
 # ----------------------------------------------------------------------------------------------------------------

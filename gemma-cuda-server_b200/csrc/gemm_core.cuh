@@ -32,10 +32,14 @@
 
 namespace nvfp4b {
 
-// Operand kinds: NVF4 = e2m1 codes with e4m3 block scales (kind::mxf4nvf4, K = 64 per MMA); BF16 = plain bf16
+// Operand kinds: NVF4 = e2m1 codes with an e4m3 scale per 16 (kind::mxf4nvf4, K = 64 per MMA); MXF4 = e2m1 codes with
+// an e8m0 scale per 32 (kind::mxf4, K = 64 per MMA, so one scale tile serves two MMAs); BF16 = plain bf16
 // (kind::f16, K = 16 per MMA, no scales).  Either way one MMA consumes 32 bytes of each operand row, so a K-tile
 // of 128 bytes is four MMAs and the shared-memory descriptors advance by 32 bytes per MMA.
-enum class Kind { NVF4, BF16 };
+enum class Kind { NVF4, MXF4, BF16 };
+
+// 512-byte scale tiles (128 rows x 4 blocks) along one K-tile.
+constexpr int sf_tiles_of(Kind k) { return k == Kind::NVF4 ? 4 : k == Kind::MXF4 ? 2 : 0; }
 
 // TMEM scale slots: one per smem stage.  The copier warps fill slot s from stage s as soon as the stage's loads
 // land, so they run ahead of the MMAs by up to STAGES - 1 K-tiles; a slot is free again when its stage is (the
@@ -45,16 +49,17 @@ struct KCfg {
     static constexpr int EPI_SMEM = EPI_SMEM_;           // extra shared memory handed to the epilogue policy
     static constexpr int BM = 128, BN = BN_, STAGES = STAGES_, ACC_BUFS = ACC_BUFS_, EPI_WARPS = EPI_WARPS_;
     static constexpr Kind KIND = KIND_;
-    static constexpr bool SCALED = KIND_ == Kind::NVF4;
+    static constexpr int SF_TILES = sf_tiles_of(KIND_);
+    static constexpr bool SCALED = SF_TILES > 0;
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;  // warps 0-3 control, 4.. epilogue
     static constexpr int KT_BYTES = 128;                 // one K-tile = 128 bytes per row (256 e2m1 or 64 bf16)
     static constexpr int A_BYTES = BM * KT_BYTES;        // 16 KB
     static constexpr int B_BYTES = BN * KT_BYTES;
-    static constexpr int SFA_BYTES = SCALED ? 4 * 512 : 0;   // 4 K-steps of 64 x one 128-row scale tile
+    static constexpr int SFA_BYTES = SF_TILES * 512;     // the scale tiles of 128 rows along the K-tile
     static constexpr int SFB_TILES = BN / 128;
-    static constexpr int SFB_BYTES = SCALED ? SFB_TILES * 4 * 512 : 0;
+    static constexpr int SFB_BYTES = SFB_TILES * SF_TILES * 512;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
-    static constexpr int SF_COLS_A = SCALED ? 16 : 0, SF_COLS_B = SCALED ? 4 * (BN / 32) : 0;
+    static constexpr int SF_COLS_A = 4 * SF_TILES, SF_COLS_B = SF_TILES * (BN / 32);
     static constexpr int SF_COL0 = ACC_BUFS * BN;
     static constexpr int TMEM_COLS = 512;
     static constexpr int SF_SLOTS = STAGES;
@@ -87,9 +92,20 @@ struct CoreParams {
     int* err;          // device error word (runtime.cu), written when a bounded wait expires
     const uint8_t* sfa;
     const uint8_t* sfb;
-    int tile_cols;     // number of 32-byte MMA K-steps along K (NVF4: = scale tiles along K = ceil(K/64))
+    int tile_cols;     // scale tiles along K; NVF4 (ceil(K/64)) and BF16: also the 32-byte MMA K-steps
     int k_tiles;       // 128-byte K-tiles
+    int mx_steps = 0;  // MXF4 only: MMA K-steps along K, ceil(K/64) (two per scale tile)
 };
+
+// MMA K-steps and scale tiles of K-tile kt.
+template <class C>
+__device__ __forceinline__ int k_steps(const CoreParams& cp, int kt) {
+    return min(4, (C::KIND == Kind::MXF4 ? cp.mx_steps : cp.tile_cols) - 4 * kt);
+}
+template <class C>
+__device__ __forceinline__ int sf_tiles(const CoreParams& cp, int kt) {
+    return min(C::SF_TILES, cp.tile_cols - C::SF_TILES * kt);
+}
 
 // ---------------------------------------------------------------------------------------------------------------
 // Scheduler policies
@@ -195,14 +211,14 @@ template <int BN>
 __device__ __forceinline__ void sched_init(GroupedSched<BN>& s) { s.init(); }
 
 // Scale copies of one K-tile, split between the two copier warps.  BN = 256: warp p copies B scale tile p for every
-// K-step and the A tile of the K-steps j with j % 2 == p (6 + 6 copies); BN = 128: warp 0 copies A, warp 1 B.  Each
-// warp then reads one 2 KB run of shared memory per B tile and writes its own TMEM columns; this split measured
+// scale tile j along K and the A tile of those with j % 2 == p (6 + 6 copies with NVF4, 3 + 3 with MXF4); BN = 128:
+// warp 0 copies A, warp 1 B.  Each warp then reads one run of shared memory per B tile and writes its own TMEM columns; this split measured
 // about 20% faster than dealing the copies out one by one.
 template <class C, bool PAIR>
-__device__ __forceinline__ void issue_scale_copies(int part, int nks, uint32_t sfa_col, uint32_t sfb_col,
+__device__ __forceinline__ void issue_scale_copies(int part, int tiles, uint32_t sfa_col, uint32_t sfb_col,
                                                    uint32_t sfa_base, uint32_t sfb_base) {
     using namespace sm100;
-    for (int j = 0; j < nks; ++j) {
+    for (int j = 0; j < tiles; ++j) {
         const bool do_a = C::BN == 256 ? (j & 1) == part : part == 0;
         const bool do_b = C::BN == 256 || part == 1;
         const int h = C::BN == 256 ? part : 0;
@@ -212,7 +228,7 @@ __device__ __forceinline__ void issue_scale_copies(int part, int nks, uint32_t s
         }
         if (do_b) {
             const uint32_t col = sfb_col + (C::BN / 32) * j + 4 * h;
-            const uint64_t d = desc_sf_32x16(sfb_base + h * 2048 + j * 512);
+            const uint64_t d = desc_sf_32x16(sfb_base + h * (C::SF_TILES * 512) + j * 512);
             if constexpr (PAIR) tmem_cp_32x128b_x4_pair(col, d);
             else tmem_cp_32x128b_x4(col, d);
         }
@@ -270,9 +286,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 const TileInfo ti = sched.tile(t);
                 for (int kt = ti.kt0; kt < ti.kt1; ++kt) {
                     if (!mbar_wait(&empty[stage], phase ^ 1u, sflag, kErrTimeoutProducer)) { ok = false; break; }
-                    const int ks0 = kt * 4;
-                    const int nks = min(4, cp.tile_cols - ks0);
-                    const uint32_t sf_bytes = C::SCALED ? (uint32_t)nks * 512u : 0u;
+                    const int ks0 = kt * C::SF_TILES;
+                    const uint32_t sf_bytes = C::SCALED ? (uint32_t)sf_tiles<C>(cp, kt) * 512u : 0u;
                     mbar_arrive_expect_tx(&full[stage], (uint32_t)(C::A_BYTES + C::B_BYTES) +
                                                             sf_bytes * (1u + (uint32_t)ti.sfb_tiles));
                     tma_load_2d(sA + stage * C::A_BYTES, &tma_a, &full[stage], kt * C::KT_BYTES, ti.a_row);
@@ -281,7 +296,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                         bulk_load(sSFA + stage * C::SFA_BYTES,
                                   cp.sfa + ((long long)ti.mb * cp.tile_cols + ks0) * 512, sf_bytes, &full[stage]);
                         for (int h = 0; h < ti.sfb_tiles; ++h)
-                            bulk_load(sSFB + stage * C::SFB_BYTES + h * 2048,
+                            bulk_load(sSFB + stage * C::SFB_BYTES + h * (C::SF_TILES * 512),
                                       cp.sfb + ((long long)(ti.sfb_tile0 + h) * cp.tile_cols + ks0) * 512, sf_bytes,
                                       &full[stage]);
                     }
@@ -299,27 +314,34 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             const uint32_t sfb_col = sfa_col + C::SF_COLS_A;
             for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
                 const TileInfo ti = sched.tile(t);
-                const uint32_t idesc = C::SCALED ? idesc_nvf4(C::BM, ti.n_mma) : idesc_bf16(C::BM, ti.n_mma);
+                const uint32_t idesc = C::KIND == Kind::NVF4   ? idesc_nvf4(C::BM, ti.n_mma)
+                                       : C::KIND == Kind::MXF4 ? idesc_mxf4(C::BM, ti.n_mma)
+                                                               : idesc_bf16(C::BM, ti.n_mma);
                 if (!mbar_wait(&tempty[abuf], aphase ^ 1u, sflag, kErrTimeoutMma)) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem + (uint32_t)(abuf * C::BN);
                 for (int kt = ti.kt0; kt < ti.kt1; ++kt) {
                     if (!mbar_wait(&full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
                     tc_fence_after();
-                    const int nks = min(4, cp.tile_cols - kt * 4);
+                    const int nks = k_steps<C>(cp, kt);
                     const uint32_t a_base = smem_u32(sA + stage * C::A_BYTES);
                     const uint32_t b_base = smem_u32(sB + stage * C::B_BYTES);
-                    const uint32_t sfa_base = smem_u32(sSFA + stage * C::SFA_BYTES);
-                    const uint32_t sfb_base = smem_u32(sSFB + stage * C::SFB_BYTES);
                     const uint32_t acc0 = kt != ti.kt0 ? 1u : 0u;
                     if constexpr (C::SCALED) {
                         if (!mbar_wait(&sf_full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
                         tc_fence_after();
                         const uint32_t so = (uint32_t)(stage * (C::SF_COLS_A + C::SF_COLS_B));
-                        for (int j = 0; j < nks; ++j)
-                            mma_nvf4(d_tmem, desc_kmajor_sw128(a_base + 32 * j), desc_kmajor_sw128(b_base + 32 * j),
-                                     idesc, sfa_col + so + 4 * j, sfb_col + so + (C::BN / 32) * j,
-                                     (acc0 | j) != 0 ? 1u : 0u);
+                        for (int j = 0; j < nks; ++j) {
+                            const uint64_t ad = desc_kmajor_sw128(a_base + 32 * j);
+                            const uint64_t bd = desc_kmajor_sw128(b_base + 32 * j);
+                            const uint32_t acc = (acc0 | j) != 0 ? 1u : 0u;
+                            if constexpr (C::KIND == Kind::MXF4)
+                                mma_mxf4(d_tmem, ad, bd, idesc | ((j & 1) ? kMxScaleId2 : 0u),
+                                         sfa_col + so + 4 * (j >> 1), sfb_col + so + (C::BN / 32) * (j >> 1), acc);
+                            else
+                                mma_nvf4(d_tmem, ad, bd, idesc, sfa_col + so + 4 * j, sfb_col + so + (C::BN / 32) * j,
+                                         acc);
+                        }
                     } else {
                         for (int j = 0; j < nks; ++j)
                             mma_bf16(d_tmem, desc_kmajor_sw128(a_base + 32 * j), desc_kmajor_sw128(b_base + 32 * j),
@@ -348,7 +370,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                     if (!mbar_wait(&full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t so = (uint32_t)(stage * (C::SF_COLS_A + C::SF_COLS_B));
-                    issue_scale_copies<C, false>(part, min(4, cp.tile_cols - kt * 4), sfa_col + so, sfb_col + so,
+                    issue_scale_copies<C, false>(part, sf_tiles<C>(cp, kt), sfa_col + so, sfb_col + so,
                                                  smem_u32(sSFA + stage * C::SFA_BYTES),
                                                  smem_u32(sSFB + stage * C::SFB_BYTES));
                     tc_commit(&sf_full[stage]);
@@ -409,20 +431,22 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 //                     CTAs' epilogues.  (warp 1 of the peer only allocates TMEM.)
 //   warps 2-3 (leader) scale copies for the pair (cta_group::2), into one TMEM scale slot per smem stage.
 //   warps 4.. (both)  epilogue of the CTA's 128 rows; one arrival per warp on the leader's accumulator-empty barrier.
-template <int STAGES_, int EPI_WARPS_, int EPI_SMEM_ = 0>
+template <int STAGES_, int EPI_WARPS_, int EPI_SMEM_ = 0, Kind KIND_ = Kind::NVF4>
 struct PairCfg {
     static constexpr int EPI_SMEM = EPI_SMEM_;
+    static constexpr Kind KIND = KIND_;
+    static constexpr int SF_TILES = sf_tiles_of(KIND_);
     static constexpr int BM = 128, PAIR_M = 256, BN = 256, STAGES = STAGES_, ACC_BUFS = 1, EPI_WARPS = EPI_WARPS_;
     static constexpr bool SCALED = true;
     static constexpr int THREADS = 128 + 32 * EPI_WARPS;     // warps 0-3 control, 4.. epilogue
     static constexpr int KT_BYTES = 128;
     static constexpr int A_BYTES = BM * KT_BYTES;             // 16 KB: this CTA's 128 rows
     static constexpr int B_BYTES = (BN / 2) * KT_BYTES;       // 16 KB: this CTA's half of the 256 B rows
-    static constexpr int SFA_BYTES = 4 * 512;                 // one 128-row scale tile, 4 K-steps
-    static constexpr int SFB_BYTES = 2 * 4 * 512;             // both 128-row scale tiles of B
+    static constexpr int SFA_BYTES = SF_TILES * 512;          // the scale tiles of 128 rows along the K-tile
+    static constexpr int SFB_BYTES = 2 * SF_TILES * 512;      // both 128-row blocks of B
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
     static constexpr uint32_t PAIR_TX = 2u * STAGE_BYTES;     // bytes the leader's full barrier waits for
-    static constexpr int SF_COLS_A = 16, SF_COLS_B = 32, SF_COL0 = BN;
+    static constexpr int SF_COLS_A = 4 * SF_TILES, SF_COLS_B = 8 * SF_TILES, SF_COL0 = BN;
     static constexpr int TMEM_COLS = 512;
     static constexpr int SF_SLOTS = STAGES;
     static constexpr int COLS_PER_WARP = BN * 4 / EPI_WARPS;
@@ -458,8 +482,8 @@ struct PairDenseSched {
     }
 };
 
-// Scale tensor maps view a tile-layout scale buffer as rows of 256 bytes; the 2 KB of one 128-row tile x one
-// K-tile (4 x 512 B) is a box of 8 rows starting at row 2 * (tile_row * tile_cols + 4 * kt).
+// Scale tensor maps view a tile-layout scale buffer as rows of 256 bytes; the SF_TILES scale tiles of 128 rows x one
+// K-tile are a box of 2 * SF_TILES rows starting at row 2 * (tile_row * tile_cols + SF_TILES * kt).
 template <class C, class Sched, class Epi>
 __global__ void __launch_bounds__(C::THREADS, 1)
     nvf4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
@@ -523,11 +547,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                     tma_load_2d_pair(sA + stage * C::A_BYTES, &tma_a, fb, kt * C::KT_BYTES, a_row);
                     tma_load_2d_pair(sB + stage * C::B_BYTES, &tma_b, fb, kt * C::KT_BYTES,
                                      ti.b_row + (int)rank * (C::BN / 2));
-                    tma_load_2d_pair(sSFA + stage * C::SFA_BYTES, &tma_sfa, fb, 0, sfa_row0 + 8 * kt);
+                    tma_load_2d_pair(sSFA + stage * C::SFA_BYTES, &tma_sfa, fb, 0, sfa_row0 + 2 * C::SF_TILES * kt);
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        tma_load_2d_pair(sSFB + stage * C::SFB_BYTES + h * 2048, &tma_sfb, fb, 0,
-                                         2 * ((ti.sfb_tile0 + h) * cp.tile_cols) + 8 * kt);
+                        tma_load_2d_pair(sSFB + stage * C::SFB_BYTES + h * (C::SF_TILES * 512), &tma_sfb, fb, 0,
+                                         2 * ((ti.sfb_tile0 + h) * cp.tile_cols) + 2 * C::SF_TILES * kt);
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
@@ -546,7 +570,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             bool ok = true;
             const uint32_t sfa_col = tmem + (uint32_t)C::SF_COL0;
             const uint32_t sfb_col = sfa_col + C::SF_COLS_A;
-            const uint32_t idesc = idesc_nvf4(C::PAIR_M, C::BN);
+            const uint32_t idesc =
+                C::KIND == Kind::MXF4 ? idesc_mxf4(C::PAIR_M, C::BN) : idesc_nvf4(C::PAIR_M, C::BN);
             const uint32_t tfull_own = smem_u32(tfull), tfull_peer = mapa_shared(smem_u32(tfull), 1);
             for (int t = cluster; t < num_tiles && ok; t += clusters) {
                 const TileInfo ti = sched.tile(t);
@@ -555,16 +580,23 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 for (int kt = ti.kt0; kt < ti.kt1; ++kt) {
                     if (!mbar_wait(&full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
                     tc_fence_after();
-                    const int nks = min(4, cp.tile_cols - kt * 4);
+                    const int nks = k_steps<C>(cp, kt);
                     const uint32_t a_base = smem_u32(sA + stage * C::A_BYTES);
                     const uint32_t b_base = smem_u32(sB + stage * C::B_BYTES);
                     const uint32_t acc0 = kt != ti.kt0 ? 1u : 0u;
                     if (!mbar_wait(&sf_full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t so = (uint32_t)(stage * (C::SF_COLS_A + C::SF_COLS_B));
-                    for (int j = 0; j < nks; ++j)
-                        mma_nvf4_pair(tmem, desc_kmajor_sw128(a_base + 32 * j), desc_kmajor_sw128(b_base + 32 * j),
-                                      idesc, sfa_col + so + 4 * j, sfb_col + so + 8 * j, (acc0 | j) != 0 ? 1u : 0u);
+                    for (int j = 0; j < nks; ++j) {
+                        const uint64_t ad = desc_kmajor_sw128(a_base + 32 * j);
+                        const uint64_t bd = desc_kmajor_sw128(b_base + 32 * j);
+                        const uint32_t acc = (acc0 | j) != 0 ? 1u : 0u;
+                        if constexpr (C::KIND == Kind::MXF4)
+                            mma_mxf4_pair(tmem, ad, bd, idesc | ((j & 1) ? kMxScaleId2 : 0u),
+                                          sfa_col + so + 4 * (j >> 1), sfb_col + so + 8 * (j >> 1), acc);
+                        else
+                            mma_nvf4_pair(tmem, ad, bd, idesc, sfa_col + so + 4 * j, sfb_col + so + 8 * j, acc);
+                    }
                     const uint32_t eb = smem_u32(&empty[stage]);
                     tc_commit_pair(eb);
                     tc_commit_pair(mapa_shared(eb, 1));
@@ -591,7 +623,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                     if (!mbar_wait(&full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t so = (uint32_t)(stage * (C::SF_COLS_A + C::SF_COLS_B));
-                    issue_scale_copies<C, true>(part, min(4, cp.tile_cols - kt * 4), sfa_col + so, sfb_col + so,
+                    issue_scale_copies<C, true>(part, sf_tiles<C>(cp, kt), sfa_col + so, sfb_col + so,
                                                 smem_u32(sSFA + stage * C::SFA_BYTES),
                                                 smem_u32(sSFB + stage * C::SFB_BYTES));
                     tc_commit_pair(smem_u32(&sf_full[stage]));
@@ -643,8 +675,8 @@ int make_kmajor_map(CUtensorMap* map, const void* base, long long rows, long lon
 // Row-major byte matrix [rows, row_bytes] (row_bytes a multiple of 16) in boxes of box_bytes x box_rows, no swizzle.
 int make_rows_map(CUtensorMap* map, const void* base, long long rows, long long row_bytes, int box_bytes,
                   int box_rows);
-// Tile-layout scale buffer of `bytes` (a multiple of 512) as rows of 256 bytes, boxes of 8 rows (2 KB), no swizzle.
-int make_scale_map(CUtensorMap* map, const void* base, long long bytes);
+// Tile-layout scale buffer of `bytes` (a multiple of 512) as rows of 256 bytes, boxes of `box_rows` rows, no swizzle.
+int make_scale_map(CUtensorMap* map, const void* base, long long bytes, int box_rows);
 
 // Clusters of two that can be resident at once (0 if the query fails).
 template <class C, class Sched, class Epi>

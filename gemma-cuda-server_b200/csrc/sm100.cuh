@@ -189,6 +189,19 @@ __device__ __forceinline__ void mma_nvf4(uint32_t d_tmem, uint64_t adesc, uint64
         : "memory");
 }
 
+// The same with MXFP4 scales (e8m0 per 32 along K): the two scale bytes of a row's 64-element step are bytes
+// [id, id + 1] (id = 0 or 2, in the instruction descriptor) of the row's TMEM scale word.
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+        : "memory");
+}
+
 // D(tmem) (+)= A(smem) * B(smem)^T, bf16 operands, fp32 accumulation (kind::f16, K = 16).
 __device__ __forceinline__ void mma_bf16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                          uint32_t accumulate) {
@@ -319,6 +332,18 @@ __device__ __forceinline__ void mma_nvf4_pair(uint32_t d_tmem, uint64_t adesc, u
         : "memory");
 }
 
+// mma_nvf4_pair with MXFP4 scales (see mma_mxf4).
+__device__ __forceinline__ void mma_mxf4_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+        : "memory");
+}
+
 // Arrive once on the mbarrier at `bar_cluster` (either CTA) when the pair operations issued so far complete.
 __device__ __forceinline__ void tc_commit_pair(uint32_t bar_cluster) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster)
@@ -347,6 +372,11 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
 __host__ __device__ constexpr uint32_t idesc_nvf4(int m, int n) {
     return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+
+// kind::mxf4 block-scaled instruction descriptor: A, B = e2m1, K-major, scales ue8m0, M x N (x64), scale id 0; the odd
+// 64-element steps of a scale word add kMxScaleId2 (id 2 for A and B).
+__host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n) { return idesc_nvf4(m, n) | (1u << 23); }
+constexpr uint32_t kMxScaleId2 = (2u << 4) | (2u << 29);
 
 }  // namespace sm100
 }  // namespace nvfp4b

@@ -143,6 +143,46 @@ int nvfp4b_linear(float* out, const float* in, int M, int N, int K, const uint8_
                   const uint8_t* w_scales_tiled, float w_gscale, float a_gscale, int mode, void* workspace,
                   size_t workspace_bytes, void* stream);
 
+/* ---- MXFP4 (OCP microscaling): quantisers, GEMM ----------------------------------------------------------------
+ *
+ * The second 4-bit format of the tensor cores: e2m1 codes packed as above, one e8m0 byte per 32-element block along K,
+ * no per-tensor scale.  With A = max |x| of a block, e = max(floor(log2 A) - 2, -127), byte = e + 127, code = nearest
+ * e2m1 to x / 2^e (ties to even, saturated at 6, the sign of x kept on zeros); value = e2m1(code) * 2^e.  A block that
+ * holds a NaN, an infinity or a magnitude of 2^128 or more stores byte 0xFF (the e8m0 NaN) and codes 0: every value of
+ * it, and every product with it, is NaN.  Scales lie in the 128x4-tile layout described at the top, with b counting
+ * blocks of 32: ceil(rows/128) * ceil(K/128) tiles of 512 bytes.  K % 32 == 0 everywhere.  Since no statistic of the
+ * whole tensor is needed, a producer (nvfp4b_block_norm, nvfp4b_mx_geglu_quantize) quantises its own output.
+ * No counterpart in the reference (its checkpoint is NVFP4); checkpoints in this format load without requantisation. */
+
+/* Bytes of a tile-layout e8m0 scale buffer for an [outer, K] operand (0 for outer or K <= 0). */
+size_t nvfp4b_mx_scale_buffer_bytes(int outer, int K);
+
+/* Device relayout of logical e8m0 scales [outer, K/32] into the tile layout (padding zeroed). */
+int nvfp4b_mx_swizzle_scales(const uint8_t* logical, uint8_t* swizzled, int outer, int K, void* stream);
+
+/* Quantise x [M, K] (rows `ldx` elements apart, ldx * element size a multiple of 16 bytes) to codes [M, K/2] and
+ * tile-layout scales (fully written, padding zero).  All pointers 16-byte aligned. */
+int nvfp4b_mx_quantize_bf16(const void* x, long long ldx, int M, int K, uint8_t* codes, uint8_t* scales, void* stream);
+int nvfp4b_mx_quantize_f32(const float* x, long long ldx, int M, int K, uint8_t* codes, uint8_t* scales,
+                           void* stream);
+
+/* Gated activation straight to MXFP4: h[m, i] = gelu_tanh(x[m, i]) * x[m, I + i] of bf16 rows [gate (I) | up (I)],
+ * rows `ld` elements apart (ld >= 2 I), codes [M, I/2] + tile-layout scales of h.  The codes and scales are those of h
+ * evaluated in float64 (the activation of the reference's kernels/elementwise.cu:44-47). */
+int nvfp4b_mx_geglu_quantize(const void* gate_up, long long ld, int M, int I, uint8_t* codes, uint8_t* scales,
+                             void* stream);
+
+/* The values of codes [M, K/2] and tile-layout scales: out [M, K] rows `ldo` elements apart, bf16 (out_f32 = 0) or fp32
+ * (1).  Exact, but for scale bytes above 252, whose largest values overflow to infinity. */
+int nvfp4b_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int K, void* out, int out_f32,
+                         long long ldo, void* stream);
+
+/* D = alpha * A @ B^T, A [M, K] and B [N, K] in MXFP4 (K-major codes, tile-layout scales), fp32 accumulation on the
+ * tensor cores (tcgen05 kind::mxf4), out_kind and ldd as for nvfp4b_gemm.  Any M, N >= 1; operands and d 16-byte
+ * aligned.  Deterministic: the same call gives the same bits. */
+int nvfp4b_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales, float alpha,
+                   int M, int N, int K, void* d, int out_kind, long long ldd, void* stream);
+
 /* ---- MoE top-k grouped expert FFN (replaces the router and expert kernels of src/forward.cu:193-321 and the
  *      orchestration of moe(), src/forward.cu:516-553) ------------------------------------------------------------
  *

@@ -1,0 +1,84 @@
+"""CPU checks of the MXFP4 operators: the oracle against the format's definition, and every refusal that is made before
+the device is touched."""
+import numpy as np
+import pytest
+import torch
+
+import mx_oracle as mx
+from __graft_entry__ import load_package
+
+
+def test_oracle_rounds_to_nearest_even_codes():
+    # e = 0 throughout: the block maximum is 4
+    x = np.zeros((1, 32))
+    x[0, :12] = [4.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, -0.25, -0.2500001, 0.7499999, -3.5000001, -0.0]
+    codes, byte = mx.quantize(x)
+    assert byte.tolist() == [[127]]
+    assert mx.dequantize(codes, byte)[0, :12].tolist() == [4, 0, 1, 1, 2, 2, 4, 0, -0.5, 0.5, -4, 0]
+    nib = np.stack([codes & 15, codes >> 4], -1).reshape(1, 32)
+    assert nib[0, 7] == 8 and nib[0, 11] == 8                 # the sign is kept on zeros
+
+
+def test_oracle_scale_bytes():
+    x = np.zeros((6, 32))
+    x[0, 3] = 7.999
+    x[1, 3] = 2.0 ** -140
+    x[2, 3] = 2.0 ** 127
+    x[3, 3] = 2.0 ** 128
+    x[4, 3] = np.nan
+    _, byte = mx.quantize(x)
+    assert byte[:, 0].tolist() == [127, 0, 252, 255, 255, 0]
+    codes, byte = mx.quantize(x[:1])
+    assert mx.dequantize(codes, byte)[0, 3] == 6.0            # saturated
+
+
+def test_oracle_error_of_a_block_is_bounded():
+    x = np.random.default_rng(0).standard_normal((64, 256))
+    v = mx.dequantize(*mx.quantize(x))
+    amax = np.abs(x.reshape(64, -1, 32)).max(2).repeat(32, 1)
+    # half the widest step of the grid is 1, and saturation loses less than 2, of a block maximum of at least 4
+    assert (np.abs(v - x) <= amax / 2).all()
+
+
+def test_scale_buffer_bytes():
+    p = load_package()
+    for rows, k in [(1, 32), (128, 128), (129, 160), (8192, 2816), (0, 32), (4, 0)]:
+        want = mx.scale_buffer_bytes(rows, k) if rows and k else 0
+        assert p.mx_scale_buffer_bytes(rows, k) == want == p._mx_sigs().nvfp4b_mx_scale_buffer_bytes(rows, k)
+
+
+def test_c_refusals():
+    L = load_package()._mx_sigs()
+    q, g, dq, mm = (L.nvfp4b_mx_quantize_bf16, L.nvfp4b_mx_geglu_quantize, L.nvfp4b_mx_dequantize, L.nvfp4b_mx_gemm)
+    assert q(None, 64, 4, 64, 16, 16, None) == -3
+    assert q(16, 64, 0, 64, 16, 16, None) == -1               # no rows
+    assert q(16, 48, 4, 48, 16, 16, None) == -1               # K % 32
+    assert q(16, 32, 4, 64, 16, 16, None) == -1               # pitch below the width
+    assert q(8, 64, 4, 64, 16, 16, None) == -2
+    assert q(16, 68, 4, 64, 16, 16, None) == -2               # pitch not a multiple of 16 bytes
+    assert L.nvfp4b_mx_quantize_f32(16, 66, 4, 64, 16, 16, None) == -2
+    assert g(16, 64, 4, 64, 16, 16, None) == -1               # pitch below 2 I
+    assert g(16, 128, 4, 0, 16, 16, None) == -1
+    assert g(16, 128, 4, 64, 16, None, None) == -3
+    assert dq(16, 16, 4, 64, 16, 2, 64, None) == -7
+    assert dq(16, 16, 4, 64, 8, 0, 64, None) == -2
+    assert dq(16, 16, 4, 64, 16, 1, 62, None) == -1
+    assert mm(16, 16, 16, 16, 1.0, 4, 4, 48, 16, 0, 4, None) == -1
+    assert mm(16, 16, 16, 16, 1.0, 0, 4, 64, 16, 0, 4, None) == -1
+    assert mm(16, 16, 16, None, 1.0, 4, 4, 64, 16, 0, 4, None) == -3
+    assert mm(16, 16, 16, 16, 1.0, 4, 4, 64, 16, 5, 4, None) == -7
+    assert mm(16, 16, 16, 16, 1.0, 4, 4, 64, 16, 1, 3, None) == -1   # column-major pitch below M
+    assert mm(16, 16, 16, 16, 1.0, 4, 4, 64, 8, 0, 4, None) == -2
+    assert L.nvfp4b_mx_swizzle_scales(16, 16, 4, 48, None) == -1
+
+
+def test_python_refusals():
+    p = load_package()
+    with pytest.raises(ValueError, match="CUDA"):
+        p.mx_quantize(torch.zeros(4, 64, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="dtype"):
+        p.mx_quantize(torch.zeros(4, 64, dtype=torch.float16))
+    with pytest.raises(ValueError, match="shape"):
+        p.mx_quantize(torch.zeros(64))
+    with pytest.raises(ValueError, match="CUDA"):
+        p.mx_gemm(*[torch.zeros(4, 32, dtype=torch.uint8)] * 4)

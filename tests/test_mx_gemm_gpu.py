@@ -1,0 +1,162 @@
+"""MXFP4 GEMM on the GPU against the float64 product of the operands' values.
+
+Tolerance: the output rounding (half a step: 2^-8 bf16, 2^-24 fp32, relative) plus fp32 accumulation -- every 64-element
+MMA step rounds its own sum and the running sum, each by at most 2^-23 of S = sum |a b| (truncation), so
+2 (steps + 1) 2^-23 S in all, plus the joins of a split K, at most 8 more."""
+import numpy as np
+import pytest
+import torch
+
+import mx_oracle as mx
+from gpu_util import require_gpu
+
+pytestmark = pytest.mark.gpu
+
+KINDS = ["bf16", "f32_col", "f32"]          # OUT_BF16_ROWMAJOR, OUT_F32_COLMAJOR, OUT_F32_ROWMAJOR
+
+
+def _operand(rows, k, seed, spread=3):
+    rng = np.random.default_rng(seed)
+    codes = rng.integers(0, 256, (rows, k // 2), dtype=np.uint8)
+    byte = rng.integers(127 - spread, 128 + spread, (rows, k // 32)).astype(np.uint8)
+    return codes, byte
+
+
+def _dev(codes, byte, k):
+    return torch.from_numpy(codes).cuda(), torch.from_numpy(mx.tile_scales(byte, k)).cuda()
+
+
+def _close(got, a, b, k, half, alpha=1.0):
+    ref, s = alpha * (a @ b.T), abs(alpha) * (np.abs(a) @ np.abs(b).T)
+    tol = half * np.abs(ref) + 2.0 * (-(-k // 64) + 9) * 2.0 ** -23 * s
+    bad = ~(np.abs(got - ref) <= tol)
+    assert not bad.any(), (int(bad.sum()), float(np.abs(got - ref).max()), np.argwhere(bad)[:4].tolist())
+
+
+def _gemm(p, A, B, m, n, kind, **kw):
+    out_kind = KINDS.index(kind)
+    shape = (n, m) if kind == "f32_col" else (m, n)
+    out = torch.full(shape, float("nan"), dtype=torch.bfloat16 if kind == "bf16" else torch.float32, device="cuda")
+    got = p.mx_gemm(*A, *B, out=out, out_kind=out_kind, **kw)
+    torch.cuda.synchronize()
+    assert got is out and p.read_device_error() == 0
+    g = got.double().cpu().numpy()
+    return g.T if kind == "f32_col" else g
+
+
+SIZES = [(1, 1, 32), (1, 2816, 2816), (2, 129, 64), (3, 4224, 96), (8, 130, 2112), (15, 1000, 160), (16, 2048, 2048),
+         (17, 257, 288), (31, 704, 2816), (33, 96, 1056), (64, 2816, 704), (65, 500, 352), (100, 8448, 2816),
+         (127, 255, 480), (128, 512, 4096), (129, 129, 32), (200, 333, 2848), (256, 256, 256), (257, 700, 544),
+         (333, 2001, 1056), (512, 2816, 2112), (640, 1, 320)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("kind", KINDS)
+def test_gemm_vs_float64(m, n, k, kind):
+    p = require_gpu()
+    a, b = _operand(m, k, m + k), _operand(n, k, n + k + 1)
+    got = _gemm(p, _dev(*a, k), _dev(*b, k), m, n, kind)
+    _close(got, mx.dequantize(*a), mx.dequantize(*b), k, 2.0 ** -8 if kind == "bf16" else 2.0 ** -24)
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 300, 416), (200, 300, 416)])
+def test_alpha_and_strided_output(m, n, k):
+    p = require_gpu()
+    a, b = _operand(m, k, 3), _operand(n, k, 4)
+    for kind, half in [("bf16", 2.0 ** -8), ("f32", 2.0 ** -24), ("f32_col", 2.0 ** -24)]:
+        r, c = (n, m) if kind == "f32_col" else (m, n)
+        for pad in (1, 8):                       # a pitch that allows wide stores, and one that does not
+            wide = torch.full((r, c + pad), 5.0, dtype=torch.bfloat16 if kind == "bf16" else torch.float32, device="cuda")
+            p.mx_gemm(*_dev(*a, k), *_dev(*b, k), out=wide[:, :c], out_kind=KINDS.index(kind), alpha=-0.375)
+            got = wide[:, :c].double().cpu().numpy()
+            _close(got.T if kind == "f32_col" else got, mx.dequantize(*a), mx.dequantize(*b), k, half, alpha=-0.375)
+            assert (wide[:, c:] == 5.0).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 200, 96), (40, 200, 96), (300, 200, 96)])
+def test_scale_bytes_over_their_range(m, n, k):
+    """Every exponent from the smallest to large ones, opposite in A and B so that the products stay in range; a NaN scale
+    makes exactly its row or column NaN."""
+    p = require_gpu()
+    rng = np.random.default_rng(m)
+    a, b = _operand(m, k, 5), _operand(n, k, 6)
+    shift = rng.integers(0, 240, k // 32)
+    a = (a[0], np.broadcast_to(shift, a[1].shape).astype(np.uint8))
+    b = (b[0], np.broadcast_to(246 - shift, b[1].shape).astype(np.uint8))
+    got = _gemm(p, _dev(*a, k), _dev(*b, k), m, n, "f32")
+    _close(got, mx.dequantize(*a), mx.dequantize(*b), k, 2.0 ** -24)
+    an, bn = a[1].copy(), b[1].copy()
+    an[m // 2, 1], bn[n - 1, 2] = 255, 255
+    nan = _gemm(p, _dev(a[0], an, k), _dev(b[0], bn, k), m, n, "f32")
+    hit = np.zeros((m, n), bool)
+    hit[m // 2], hit[:, n - 1] = True, True
+    assert np.isnan(nan[hit]).all()
+    assert np.array_equal(nan[~hit], got[~hit])
+
+
+def test_same_bits_every_time_and_for_every_row_count():
+    """Two calls give the same bits, and so do two graph replays on fresh contents of the same buffers."""
+    p = require_gpu()
+    for m, n, k in [(1, 2816, 2816), (16, 4224, 2816), (300, 1000, 1056)]:
+        a, b = _dev(*_operand(m, k, 7), k), _dev(*_operand(n, k, 8), k)
+        one = p.mx_gemm(*a, *b, out_kind=p.OUT_F32_ROWMAJOR)
+        assert torch.equal(one, p.mx_gemm(*a, *b, out_kind=p.OUT_F32_ROWMAJOR))
+        graph, out = torch.cuda.CUDAGraph(), torch.empty_like(one)
+        with torch.cuda.graph(graph):
+            p.mx_gemm(*a, *b, out=out, out_kind=p.OUT_F32_ROWMAJOR)
+        for _ in range(2):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, one)
+
+
+def test_two_streams_at_once():
+    p = require_gpu()
+    m, n, k = 16, 8448, 2816
+    ops = [(_dev(*_operand(m, k, i), k), _dev(*_operand(n, k, 20 + i), k)) for i in range(2)]
+    want = [p.mx_gemm(*a, *b) for a, b in ops]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ops]
+    got = [[p.mx_gemm(*a, *b, stream=s) for _ in range(8)] for (a, b), s in zip(ops, streams)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
+
+
+def test_full_size_sampled():
+    """The largest prefill of the GEMM benchmark; float64 on sampled rows and all columns."""
+    p = require_gpu()
+    m, n, k = 8192, 14336, 4096
+    g = torch.Generator("cuda").manual_seed(0)
+    A = p.mx_quantize(torch.randn(m, k, generator=g, device="cuda").bfloat16())
+    B = p.mx_quantize((0.02 * torch.randn(n, k, generator=g, device="cuda")).bfloat16())
+    got = p.mx_gemm(*A, *B)
+    torch.cuda.synchronize()
+    assert p.read_device_error() == 0
+    rows = torch.tensor([0, 1, 127, 128, 255, 256, 4095, 5000, 8191], device="cuda")
+    a = p.mx_dequantize(*A, dtype=torch.float32)[rows].double()
+    b = p.mx_dequantize(*B, dtype=torch.float32).double()
+    _close(got[rows].double().cpu().numpy(), a.cpu().numpy(), b.cpu().numpy(), k, 2.0 ** -8)
+
+
+def test_refusals():
+    p = require_gpu()
+    a, b = _dev(*_operand(4, 64, 1), 64), _dev(*_operand(8, 64, 2), 64)
+    with pytest.raises(ValueError, match="shape"):
+        p.mx_gemm(*a, *_dev(*_operand(8, 96, 2), 96))
+    with pytest.raises(ValueError, match="scales"):
+        p.mx_gemm(a[0], a[1][:256], *b)
+    with pytest.raises(ValueError, match="out"):
+        p.mx_gemm(*a, *b, out=torch.empty(4, 8, device="cuda"))
+    with pytest.raises(ValueError, match="out_kind"):
+        p.mx_gemm(*a, *b, out_kind=3)
+    with pytest.raises(ValueError, match="multiple of 32"):
+        p.mx_gemm(a[0][:, :24].contiguous(), a[1], b[0][:, :24].contiguous(), b[1])
+    with pytest.raises(p.NvFp4Error, match="SHAPE"):
+        p.mx_gemm(a[0][:0], a[1], *b)
+    with pytest.raises(p.NvFp4Error, match="ALIGN"):
+        p.mx_gemm(*a, *b, out=torch.empty(40, dtype=torch.bfloat16, device="cuda")[1:33].view(4, 8))
+    with pytest.raises(ValueError, match="codes"):
+        p.mx_quantize(torch.zeros(4, 64, device="cuda"), codes=torch.empty(4, 16, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(p.NvFp4Error, match="ALIGN"):
+        p.mx_quantize(torch.zeros(4, 66, device="cuda")[:, :64])
