@@ -10,8 +10,8 @@ Two layers:
   ``nvfp4_swizzle_scales``, ``nvfp4_gemm``, ``w4a16_gemm``, ``fp4_gemv`` -- device pointers as torch tensors;
 * tensor-level helpers used by the tests and the benchmark: ``quantize``, ``amax``, ``gemm``, ``linear``, the MoE
   layer (``moe_route``, ``moe_forward`` with its chained and fused-norm forms, ``moe_layer`` with the router fused
-  in, ``MoeExperts``), the MXFP4 operators (``mx_quantize``, ``mx_geglu_quantize``, ``mx_dequantize``, ``mx_gemm``),
-  and the
+  in, ``MoeExperts``), the MXFP4 operators (``mx_quantize``, ``mx_geglu_quantize``, ``mx_dequantize``, ``mx_gemm``)
+  with the norms around a block that quantise their own output (``block_norm``), and the
   expert-parallel entry points (``ep_*`` over NCCL slots, ``ep_p2p_*`` over peer memory with the ``ipc_*`` set-up
   helpers; ``expert_parallel.py`` orchestrates them).
 """
@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+from typing import NamedTuple
 
 import torch
 
@@ -235,10 +236,20 @@ def hbm_read_stream(buf: torch.Tensor, rows: int, row_bytes: int) -> None:
 
 
 # ----------------------------------------------------------------------------------------------------------------
-# MXFP4 (include/nvfp4_b200.h: nvfp4b_mx_*)
+# MXFP4 and the block norm (include/nvfp4_b200.h: nvfp4b_mx_*, nvfp4b_block_norm)
 # ----------------------------------------------------------------------------------------------------------------
 # These check what they are given before anything is launched (ValueError), run on the tensors' device whatever the
 # current one is, and allocate outputs that are not given on the stream that the call runs on.
+
+class _BlockNormArgs(ctypes.Structure):
+    _fields_ = [("T", ctypes.c_int), ("H", ctypes.c_int), ("resid_f32", ctypes.c_int), ("y_f32", ctypes.c_int),
+                ("resid", _P), ("y", _P), ("ld_resid", ctypes.c_longlong), ("ld_y", ctypes.c_longlong),
+                ("post_norm", ctypes.c_int), ("gate_f32", ctypes.c_int), ("post_weight", _P), ("gate", _P),
+                ("gate_row_stride", ctypes.c_longlong), ("gate_col_stride", ctypes.c_int), ("scale", ctypes.c_float),
+                ("eps", ctypes.c_float), ("resid_out_f32", ctypes.c_int), ("resid_out", _P),
+                ("ld_resid_out", ctypes.c_longlong), ("norm_weight", _P), ("out", _P), ("ld_out", ctypes.c_longlong),
+                ("amax", _P), ("codes", _P), ("scales", _P)]
+
 
 def _mx_sigs():
     L = lib()
@@ -254,6 +265,7 @@ def _mx_sigs():
         "nvfp4b_mx_dequantize": ([_P, _P, ctypes.c_int, ctypes.c_int, _P, ctypes.c_int, ll, _P], ctypes.c_int),
         "nvfp4b_mx_gemm": ([_P, _P, _P, _P, ctypes.c_float, ctypes.c_int, ctypes.c_int, ctypes.c_int, _P,
                             ctypes.c_int, ll, _P], ctypes.c_int),
+        "nvfp4b_block_norm": ([ctypes.POINTER(_BlockNormArgs), _P], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         f = getattr(L, name)
@@ -396,6 +408,94 @@ def mx_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: 
     _launch("mx_gemm", _mx_sigs().nvfp4b_mx_gemm, dev, stream, _ptr(a), _ptr(a_scales), _ptr(b), _ptr(b_scales),
             float(alpha), M, N, K, _ptr(out), out_kind, ldd)
     return out
+
+
+class BlockNorm(NamedTuple):
+    """What ``block_norm`` wrote (None = not asked for)."""
+    resid: torch.Tensor | None
+    out: torch.Tensor | None
+    amax: torch.Tensor | None
+    codes: torch.Tensor | None
+    scales: torch.Tensor | None
+
+
+_FLOATS = (torch.bfloat16, torch.float32)
+
+
+def block_norm(resid: torch.Tensor | None = None, norm_weight: torch.Tensor | None = None, eps: float = 1e-6,
+               y: torch.Tensor | None = None, post_weight: torch.Tensor | None = None, post_norm: bool | None = None,
+               gate: torch.Tensor | None = None, scale: float = 1.0, resid_out: torch.Tensor | None = None,
+               out: torch.Tensor | None = None, amax: torch.Tensor | None = None, codes: torch.Tensor | None = None,
+               scales: torch.Tensor | None = None, mx: bool = False, stream=None) -> BlockNorm:
+    """The norms around a block, with its gate, residual and residual scale, in one pass over the rows:
+
+        n = [rms(y)] * post_weight;  r = scale * (resid + gate * n) -> resid_out;  z = rms(r) * norm_weight
+
+    resid, y: bf16 or fp32 [T, H] (either may be None); the weights bf16 [H] (None = ones); post_norm: whether y is
+    normalised (default: with a post_weight); gate: bf16 or fp32, [H] per feature, [T, 1] per token or [T, H].
+    z goes to `out` (bf16 [T, H]; with `amax`, fp32 [1], its max |z|) and / or to MXFP4 `codes` and `scales` (mx=True
+    allocates them).  Without any of these, z is written to a new `out` if norm_weight is given, and r to a new
+    resid_out (of resid's type, or y's) if y is.  resid_out may be resid itself."""
+    x = resid if resid is not None else y
+    if x is None:
+        raise ValueError("block_norm: resid or y is needed")
+    if x.dim() != 2:
+        raise ValueError(f"block_norm: shape {tuple(x.shape)}, expected [T, H]")
+    T, H = x.shape
+    dev, a = x.device, _BlockNormArgs()
+    a.T, a.H, a.scale, a.eps = T, H, scale, eps
+    mx = mx or codes is not None or scales is not None
+    if resid is not None:
+        a.ld_resid = _rows("block_norm: resid", resid, _FLOATS, (T, H), dev)
+        a.resid, a.resid_f32 = resid.data_ptr(), resid.dtype == torch.float32
+    if y is not None:
+        a.ld_y = _rows("block_norm: y", y, _FLOATS, (T, H), dev)
+        a.y, a.y_f32 = y.data_ptr(), y.dtype == torch.float32
+        if resid_out is None and out is None and not mx and norm_weight is None:
+            resid_out = _empty((T, H), x.dtype, dev, stream)
+    elif post_weight is not None or post_norm or gate is not None:
+        raise ValueError("block_norm: post_weight, post_norm and gate need y")
+    if post_weight is not None:
+        _flat("block_norm: post_weight", post_weight, torch.bfloat16, H, dev)
+        a.post_weight = post_weight.data_ptr()
+    a.post_norm = post_weight is not None if post_norm is None else bool(post_norm)
+    if gate is not None:
+        if gate.dtype not in _FLOATS or gate.device != dev or tuple(gate.shape) not in ((H,), (T, 1), (T, H)):
+            raise ValueError(f"block_norm: gate {tuple(gate.shape)} {gate.dtype} on {gate.device}, expected bf16 or fp32 "
+                             f"[{H}], [{T}, 1] or [{T}, {H}] on {dev}")
+        cols = gate.shape[-1] > 1 or H == 1
+        if cols and gate.stride(-1) != 1:
+            raise ValueError("block_norm: gate: columns must be contiguous")
+        a.gate, a.gate_f32, a.gate_col_stride = gate.data_ptr(), gate.dtype == torch.float32, 1 if cols else 0
+        a.gate_row_stride = gate.stride(0) if gate.dim() == 2 and T > 1 else 0
+    if norm_weight is not None:
+        _flat("block_norm: norm_weight", norm_weight, torch.bfloat16, H, dev)
+        a.norm_weight = norm_weight.data_ptr()
+        if out is None and not mx:
+            out = _empty((T, H), torch.bfloat16, dev, stream)
+    if resid_out is not None:
+        a.ld_resid_out = _rows("block_norm: resid_out", resid_out, _FLOATS, (T, H), dev)
+        a.resid_out, a.resid_out_f32 = resid_out.data_ptr(), resid_out.dtype == torch.float32
+        if resid is not None and a.resid_out == a.resid and (resid_out.dtype, a.ld_resid_out) != (resid.dtype, a.ld_resid):
+            raise ValueError("block_norm: resid_out on resid with another type or pitch")
+    if out is not None:
+        a.ld_out = _rows("block_norm: out", out, (torch.bfloat16,), (T, H), dev)
+        a.out = out.data_ptr()
+        for t, ld in ((resid, a.ld_resid), (y, a.ld_y)):
+            if t is not None and a.out == t.data_ptr() and (out.dtype, a.ld_out) != (t.dtype, ld):
+                raise ValueError("block_norm: out on an input of another type or pitch")
+        if resid_out is not None and a.out == a.resid_out:
+            raise ValueError("block_norm: out on resid_out")
+    if amax is not None:
+        if out is None:
+            raise ValueError("block_norm: amax needs out")
+        _flat("block_norm: amax", amax, torch.float32, 1, dev)
+        a.amax = amax.data_ptr()
+    if mx:
+        codes, scales = _mx_buffers("block_norm", T, H, codes, scales, dev, stream)
+        a.codes, a.scales = codes.data_ptr(), scales.data_ptr()
+    _launch("block_norm", _mx_sigs().nvfp4b_block_norm, dev, stream, ctypes.byref(a))
+    return BlockNorm(resid_out, out, amax, codes, scales)
 
 
 # ----------------------------------------------------------------------------------------------------------------

@@ -183,6 +183,45 @@ int nvfp4b_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int
 int nvfp4b_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales, float alpha,
                    int M, int N, int K, void* d, int out_kind, long long ldd, void* stream);
 
+/* ---- Norms before and after a block, with its gate, residual and residual scale ------------------------------------
+ *
+ *   n = [rms(y; eps)] * post_weight      the block's output y, its norm only with post_norm = 1 (weights alone with 0)
+ *   r = scale * (resid + gate * n)       -> resid_out
+ *   z = rms(r; eps) * norm_weight        -> out (bf16) with its max |z| in *amax, and/or codes + scales (MXFP4)
+ * with rms(x; eps) = x / sqrt(mean(x^2) + eps) over the H elements of a row (the reference's rmsnorm,
+ * kernels/elementwise.cu:10-22, and the post-norms, residual and layer_scalar of moe(), src/forward.cu:546-551).  Every
+ * input is read once and r and z are taken from the unrounded values of the step before.  fp32 sums; the MXFP4 codes and
+ * scales are those of the float64 z.  *amax (zeroed by this call) is the maximum of the bf16 out, as nvfp4b_amax_bf16
+ * would find it: out and amax are what nvfp4b_quantize_bf16 takes with a dynamic scale.
+ * resid_out may be resid itself (same type and pitch), out may be y or resid where those are bf16 rows of the same pitch;
+ * no other overlap of inputs and outputs.  Rows are `ld_*` elements apart.  H % 8 == 0 (% 32 with codes). */
+#define NVFP4B_BLOCK_NORM_MAX_H 16384
+
+typedef struct nvfp4b_block_norm_args {
+    int T, H;                      /* rows, row width */
+    int resid_f32, y_f32;          /* 0 = bf16, 1 = fp32 */
+    const void* resid;             /* [T, H]; NULL = 0 (y must be given) */
+    const void* y;                 /* [T, H]; NULL = no block output: r = scale * resid, z its norm */
+    long long ld_resid, ld_y;
+    int post_norm, gate_f32;
+    const void* post_weight;       /* bf16 [H]; NULL = ones */
+    const void* gate;              /* element (t, i) at t * gate_row_stride + i * gate_col_stride; NULL = ones */
+    long long gate_row_stride;     /* 0 = the same for every row */
+    int gate_col_stride;           /* 0 = one value per row, 1 */
+    float scale, eps;
+    int resid_out_f32;
+    void* resid_out;               /* [T, H]; NULL = not written */
+    long long ld_resid_out;
+    const void* norm_weight;       /* bf16 [H]; NULL = ones */
+    void* out;                     /* bf16 [T, H]; NULL = not written */
+    long long ld_out;
+    float* amax;                   /* one fp32, with out only; NULL = not wanted */
+    uint8_t* codes;                /* [T, H/2] MXFP4 codes and their tile-layout scales; both or neither */
+    uint8_t* scales;
+} nvfp4b_block_norm_args;
+
+int nvfp4b_block_norm(const nvfp4b_block_norm_args* args, void* stream);
+
 /* ---- MoE top-k grouped expert FFN (replaces the router and expert kernels of src/forward.cu:193-321 and the
  *      orchestration of moe(), src/forward.cu:516-553) ------------------------------------------------------------
  *

@@ -1,0 +1,254 @@
+"""The block norm on the GPU against its float64 definition.
+
+MXFP4 codes and scales are equal bit for bit.  bf16 outputs: half a step (2^-8) plus the fp32 error of the value, fp32
+outputs: that error alone.  With u = 2^-24 the error of r is at most 20 u a, a = |scale| (|resid| + |gate n|) (a mean of
+squares and its root, three products, a sum and a product), that of z at most |z| (16 + 20 k) u + 20 u a |f w| with
+k = sqrt(sum a^2 / sum r^2) per row; both are taken twice here."""
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+import mx_oracle as mx
+from gpu_util import poisoned, require_gpu
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _n(t):
+    return None if t is None else t.double().cpu().numpy()
+
+
+def _want(kw):
+    """Float64 r and z, and their tolerances."""
+    names = ("resid", "norm_weight", "y", "post_weight", "gate")
+    v = {k: _n(kw.get(k)) for k in names}
+    eps, scale = float(np.float32(kw.get("eps", 1e-6))), float(np.float32(kw.get("scale", 1.0)))
+    post = kw.get("post_norm")
+    with np.errstate(over="ignore", invalid="ignore", divide="ignore"):
+        r, z = mx.block_norm(eps=eps, post_norm=post, scale=scale, **v)
+        n, _ = mx.block_norm(None, None, eps, v["y"], v["post_weight"], post, v["gate"]) if v["y"] is not None else (0, 0)
+        a = abs(scale) * (np.abs(n) + (np.abs(v["resid"]) if v["resid"] is not None else 0))
+        f = 1 / np.sqrt((r * r).mean(1, keepdims=True) + eps)
+        k = np.sqrt((a * a).sum(1, keepdims=True) / np.maximum((r * r).sum(1, keepdims=True), 1e-300))
+        w = 1.0 if v["norm_weight"] is None else np.abs(v["norm_weight"])
+        return r, z, 40 * U * a, 2 * U * (np.abs(z) * (16 + 20 * k) + 20 * a * f * w)
+
+
+def _near(got, ref, tol, dtype):
+    got = _n(got)
+    tol = tol + np.abs(ref) * (2.0 ** -8 if dtype == torch.bfloat16 else U) + 2.0 ** -133
+    ok = (np.abs(got - ref) <= tol) | (np.isnan(got) & np.isnan(ref))
+    assert ok.all(), (np.argwhere(~ok)[:4].tolist(), got[~ok][:4], ref[~ok][:4])
+
+
+def _check(p, T, H, want_mx, want_out, resid_out=None, **kw):
+    r, z, dr, dz = _want(kw)
+    out = torch.full((T, H), float("nan"), dtype=torch.bfloat16, device="cuda") if want_out else None
+    amax = torch.full((1,), -1.0, device="cuda") if want_out else None
+    codes = poisoned(T * H // 2).view(T, H // 2) if want_mx else None
+    scales = poisoned(mx.scale_buffer_bytes(T, H)) if want_mx else None
+    if resid_out is None:
+        resid_out = torch.full((T, H), float("nan"), dtype=torch.float32, device="cuda")
+    got = p.block_norm(resid_out=resid_out, out=out, amax=amax, codes=codes, scales=scales, **kw)
+    torch.cuda.synchronize()
+    _near(got.resid, r, dr, resid_out.dtype)
+    if want_out:
+        _near(out, z, dz, torch.bfloat16)
+        assert amax.item() == out.float().abs().max().item()
+    if want_mx:
+        byte, clean = mx.untile_scales(scales.cpu().numpy(), T, H)
+        ref = mx.quantize(z)
+        assert np.array_equal(byte, ref[1]) and clean
+        assert np.array_equal(codes.cpu().numpy(), ref[0])
+    return got
+
+
+def _make(T, H, seed, resid, y, post=True, gate="", std=3.0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    kw = {"norm_weight": (1 + 0.1 * rn(H)).bfloat16()}
+    if resid:
+        kw["resid"] = rn(T, H).to(resid)
+    if y:
+        kw["y"] = (std * rn(T, H)).to(y)
+        if post:
+            kw["post_weight"] = (1 + 0.1 * rn(H)).bfloat16()
+        shape = {"": None, "feature": (H,), "row": (T, 1), "full": (T, H)}[gate]
+        if shape:
+            kw["gate"] = torch.sigmoid(rn(*shape))
+    return kw
+
+
+B, F = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("T,H", [(1, 32), (1, 2816), (3, 96), (130, 160), (129, 2816), (64, 4096), (9, 4128), (5, 8224),
+                                 (2, 16384), (300, 2112)])
+@pytest.mark.parametrize("resid,y", [(B, None), (F, None), (B, B), (F, F), (B, F), (None, B)])
+def test_norm_to_mxfp4_and_bf16(T, H, resid, y):
+    p = require_gpu()
+    kw = _make(T, H, T + H, resid, y)
+    _check(p, T, H, True, False, **kw)
+    _check(p, T, H, True, True, scale=0.6, **kw)
+    _check(p, T, H, False, True, scale=-1.7, eps=1e-5, **kw)
+
+
+@pytest.mark.parametrize("T,H", [(1, 8), (5, 24), (33, 1000), (2, 5000)])
+def test_widths_of_a_multiple_of_eight(T, H):
+    p = require_gpu()
+    _check(p, T, H, False, True, **_make(T, H, H, F, B, gate="row"))
+
+
+@pytest.mark.parametrize("gate,dtype", list(itertools.product(["feature", "row", "full"], [B, F])))
+def test_gates(gate, dtype):
+    p = require_gpu()
+    kw = _make(70, 704, 5, B, B, gate=gate)
+    kw["gate"] = kw["gate"].to(dtype)
+    _check(p, 70, 704, True, True, scale=0.5, **kw)
+    kw["gate"] = torch.cat([kw["gate"], kw["gate"]], -1)[..., :kw["gate"].shape[-1]]          # strided
+    _check(p, 70, 704, True, True, scale=0.5, **kw)
+
+
+@pytest.mark.parametrize("post_norm", [True, False])
+def test_post_norm_and_weights_apart(post_norm):
+    p = require_gpu()
+    kw = _make(40, 512, 6, F, F, post=False)
+    _check(p, 40, 512, True, True, post_norm=post_norm, **kw)
+    kw["post_weight"] = kw["norm_weight"]
+    kw["norm_weight"] = None
+    _check(p, 40, 512, True, True, post_norm=post_norm, **kw)
+
+
+def test_many_rows_equal_codes():
+    """Enough elements that fp32 alone would put some on the wrong side of a rounding border."""
+    p = require_gpu()
+    for resid, y, gate in [(B, None, ""), (F, B, "row")]:
+        _check(p, 2000, 2816, True, False, **_make(2000, 2816, 11, resid, y, gate=gate))
+
+
+def test_rows_that_cancel_vanish_or_overflow():
+    """resid = -n up to rounding, zero rows, subnormal and huge rows, NaN and infinities: the float64 codes all the same."""
+    p = require_gpu()
+    T, H = 12, 160
+    kw = _make(T, H, 8, F, F)
+    r, _ = mx.block_norm(None, None, float(np.float32(1e-6)), _n(kw["y"]), _n(kw["post_weight"]))
+    kw["resid"][:4] = torch.from_numpy(-r[:4]).float().cuda()
+    kw["resid"][4], kw["y"][4] = 0, 0
+    kw["resid"][5] *= 1e-40
+    kw["y"][5] *= 1e-42
+    kw["resid"][6] *= 1e30
+    kw["y"][7] *= 1e25
+    kw["resid"][8, 3], kw["y"][9, 5], kw["resid"][10, 0] = float("nan"), float("inf"), float("-inf")
+    kw["y"][11] = 0
+    r, z, _, _ = _want(kw)
+    codes, scales = poisoned(T * H // 2).view(T, H // 2), poisoned(mx.scale_buffer_bytes(T, H))
+    out = torch.empty(T, H, dtype=B, device="cuda")
+    p.block_norm(codes=codes, scales=scales, out=out, resid_out=kw["resid"], **kw)            # in place
+    ref = mx.quantize(z)
+    byte, clean = mx.untile_scales(scales.cpu().numpy(), T, H)
+    assert np.array_equal(byte, ref[1]) and clean and np.array_equal(codes.cpu().numpy(), ref[0])
+    assert np.array_equal(np.isnan(_n(out)), np.isnan(z))
+    ok = np.isfinite(z)
+    assert (np.abs(_n(out)[ok] - z[ok]) <= np.abs(z[ok]) * 2.0 ** -7).all()
+
+
+def test_zero_eps_and_zero_rows():
+    p = require_gpu()
+    x = torch.zeros(3, 64, dtype=B, device="cuda")
+    x[1] = 2.0 ** -100
+    got = p.block_norm(x, eps=0.0, mx=True)
+    v = _n(p.mx_dequantize(got.codes, got.scales))
+    assert np.isnan(v[[0, 2]]).all() and (v[1] == 1.0).all()
+
+
+def test_in_place_strided_and_defaults():
+    p = require_gpu()
+    base = _make(50, 512, 9, B, B)
+    r, z, dr, dz = _want(base)
+    wide = torch.full((50, 1024), 3.0, dtype=B, device="cuda")
+    wide[:, :512], wide[:, 512:] = base["resid"], base["y"]
+    kw = {**base, "resid": wide[:, :512], "y": wide[:, 512:]}
+    got = p.block_norm(resid_out=kw["resid"], out=kw["y"], **kw)                              # r on resid, z on y
+    _near(got.resid, r, dr, B)
+    _near(got.out, z, dz, B)
+    only_r = p.block_norm(base["resid"], y=base["y"], post_weight=base["post_weight"])
+    assert only_r.out is None and torch.equal(only_r.resid, got.resid)
+    only_z = p.block_norm(**base)
+    assert only_z.resid is None and torch.equal(only_z.out, got.out)
+
+
+def test_amax_feeds_the_nvfp4_quantiser():
+    p = require_gpu()
+    kw = _make(200, 704, 10, F, F)
+    out, amax = torch.empty(200, 704, dtype=B, device="cuda"), torch.empty(1, device="cuda")
+    p.block_norm(out=out, amax=amax, **kw)
+    assert torch.equal(amax, p.amax(out))
+    a, b = p.quantize(out, amax_dev=amax), p.quantize(out, amax_dev=p.amax(out))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_captured_block():
+    """Two layers of a dense MXFP4 feed-forward as they are used -- norm, product, gate, product, norm -- captured into one
+    graph, replayed on new rows, against float64 with the device's codes taken as the operands."""
+    p = require_gpu()
+    T, H, I = 48, 704, 2112
+    g = torch.Generator("cuda").manual_seed(3)
+    rn = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    x, w = rn(T, H), [(1 + 0.1 * rn(H)).bfloat16() for _ in range(3)]
+    gu, dn = p.mx_quantize(0.04 * rn(2 * I, H)), p.mx_quantize(0.03 * rn(H, I))
+
+    def step():
+        first = p.block_norm(x, w[0], mx=True)
+        up = p.mx_gemm(first.codes, first.scales, *gu)
+        h = p.mx_geglu_quantize(up)
+        y = p.mx_gemm(*h, *dn)
+        return first, up, h, y, p.block_norm(x, w[2], y=y, post_weight=w[1], scale=0.9,
+                                             resid_out=torch.empty_like(x), mx=True)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first, up, h, y, last = step()
+    for seed in range(2):
+        x.copy_(rn(T, H))
+        graph.replay()
+        torch.cuda.synchronize()
+        v = lambda c: _n(p.mx_dequantize(*c, dtype=torch.float32))  # noqa: E731
+        _, z = mx.block_norm(_n(x), _n(w[0]), float(np.float32(1e-6)))
+        assert np.array_equal(v(first[3:]), mx.dequantize(*mx.quantize(z)))
+        for got, a, b in ((up, first[3:], gu), (y, h, dn)):
+            a, b = v(a), v(b)
+            s = np.abs(a) @ np.abs(b).T
+            assert (np.abs(_n(got) - a @ b.T) <= 2.0 ** -8 * np.abs(a @ b.T) + 2.0 ** -17 * s).all()
+        assert np.array_equal(v(h), mx.dequantize(*mx.quantize(mx.geglu(_n(up)[:, :I], _n(up)[:, I:]))))
+        r, z = mx.block_norm(_n(x), _n(w[2]), float(np.float32(1e-6)), _n(y), _n(w[1]), scale=float(np.float32(0.9)))
+        assert np.array_equal(v(last[3:]), mx.dequantize(*mx.quantize(z)))
+        assert np.abs(_n(last.resid) - r).max() <= 1e-5
+
+
+def test_refusals():
+    p = require_gpu()
+    x = torch.zeros(4, 64, device="cuda")
+    w = torch.ones(64, dtype=B, device="cuda")
+    for match, kw in [("resid or y", {}), ("need y", dict(resid=x, post_weight=w)), ("need y", dict(resid=x, gate=w)),
+                      ("dtype", dict(resid=x.half(), norm_weight=w)), ("norm_weight", dict(resid=x, norm_weight=w.float())),
+                      ("norm_weight", dict(resid=x, norm_weight=w[:32])), ("shape", dict(resid=x, y=x[:2])),
+                      ("gate", dict(resid=x, y=x, gate=torch.ones(4, device="cuda"))),
+                      ("contiguous", dict(resid=x, y=x, gate=torch.ones(128, device="cuda")[::2])),
+                      ("amax", dict(resid=x, mx=True, amax=torch.empty(1, device="cuda"))),
+                      ("type or pitch", dict(resid=x, y=x, resid_out=x.view(B)[:, :64])),
+                      ("multiple of 32", dict(resid=x[:, :40].contiguous(), mx=True)),
+                      ("cuda", dict(resid=x, norm_weight=w.cpu()))]:
+        with pytest.raises(ValueError, match=match):
+            p.block_norm(**kw)
+    with pytest.raises(p.NvFp4Error, match="NULL"):
+        p.block_norm(x)
+    with pytest.raises(p.NvFp4Error, match="SHAPE"):
+        p.block_norm(torch.zeros(1, 16392, device="cuda"), resid_out=torch.zeros(1, 16392, device="cuda"))
+    with pytest.raises(p.NvFp4Error, match="ALIGN"):
+        p.block_norm(torch.zeros(4, 66, device="cuda")[:, :64], w)
+    with pytest.raises(p.NvFp4Error, match="ARG"):
+        p.block_norm(x, w, eps=-1.0)

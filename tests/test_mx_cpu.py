@@ -82,3 +82,24 @@ def test_python_refusals():
         p.mx_quantize(torch.zeros(64))
     with pytest.raises(ValueError, match="CUDA"):
         p.mx_gemm(*[torch.zeros(4, 32, dtype=torch.uint8)] * 4)
+
+
+def test_block_norm_c_refusals():
+    p = load_package()
+    L, A = p._mx_sigs(), p._BlockNormArgs
+
+    def call(**kw):
+        base = dict(T=4, H=64, resid=16, ld_resid=64, resid_out=16, ld_resid_out=64, eps=1e-6, scale=1.0)
+        return L.nvfp4b_block_norm(A(**{**base, **kw}), None)
+
+    assert L.nvfp4b_block_norm(None, None) == -3
+    assert call(T=0) == -1 and call(H=60) == -1 and call(H=16392) == -1 and call(ld_resid=32) == -1
+    assert call(H=40, ld_resid=40, ld_resid_out=40, codes=16, scales=16) == -1        # H % 32 with codes
+    assert call(resid=None) == -3 and call(resid_out=None) == -3 and call(codes=16) == -3 and call(amax=16) == -3
+    assert call(resid_f32=2) == -7 and call(eps=-1.0) == -7 and call(eps=float("nan")) == -7
+    assert call(gate=16) == -7 and call(post_weight=16) == -7 and call(post_norm=1) == -7   # without y
+    assert call(y=16, ld_y=64, gate=16, gate_col_stride=2) == -7
+    assert call(y=16, ld_y=64, gate=16, gate_row_stride=-1) == -1
+    assert call(resid=8) == -2 and call(ld_resid=68) == -2 and call(norm_weight=8, out=16, ld_out=64) == -2
+    assert call(y=16, ld_y=64, gate=18, gate_f32=1) == -2
+    assert call(out=16, ld_out=64, amax=18) == -2
