@@ -1,66 +1,134 @@
 // block_norm.cu -- the norms around a transformer block, with its gate, residual and residual scale, in one pass:
 //   n = rms(y; eps) * post_w,   r = scale * (resid + gate * n),   z = rms(r; eps) * norm_w
 // r is written as the new residual; z as bf16 (with its max |.|, the dynamic scale of an NVFP4 quantiser) and/or as MXFP4
-// codes and scales.  Each input is read once and each output written once: the row stays in registers.
+// codes and scales.  Each input is read once and each output written once; DRAM bounds it at prefill sizes.
 //
-// One CTA per row, 8 consecutive elements per thread and chunk; the two sums of squares are block reductions.  The codes
-// stored are those of the float64 z: with u = 2^-24 the fp32 r is off by at most 17 u a, a = |scale| (|resid| +
-// |gate n|) (12 u for rsqrt of a mean of squares -- 8 + 5 + 5 additions, half of them after the root -- and the
-// products after it), and z by
-//   d = |f w| (20 u a + |r| (16 u + 20 u k)),  k = sqrt(sum a^2 / sum r^2),  f = 1 / rms(r)
-// (without y: r is one product, d = 20 u |z|).  Where the codes of z - d and z + d differ, or a sum of squares leaves
-// the range in which the bounds hold, the CTA redoes its row in float64.
+// Persistent CTAs, one row at a time, 8 consecutive elements per thread and chunk.  The rows of y and resid come by
+// bulk copies into a ring of two shared-memory stages, so the next row is on its way while this one goes through its
+// two or three block-wide barriers (a first version with a CTA per row and loads into registers spent its time
+// waiting: 148 us for 8192 x 2816 bf16 with a gate to MXFP4).  NCH chunks per thread: 4 at many rows (small CTAs,
+// several per SM), 1 at few (the shortest path through one row).
+//
+// The codes stored are those of the float64 z.  With u = 2^-24 a sum of squares is off by at most 17 u of itself (4
+// fused steps and a join per chunk, 3 chunk joins, 5 + 4 tree levels), 1 / rms by 10 u, r by 15 u a with a = |scale|
+// (|resid| + |gate n|), and z by
+//   d = |f w| A (28 u + 16 u k),   A = max a of the chunk,  k = sqrt(sum a^2 / sum r^2),  f = 1 / rms(r),
+// without y (r is one product) by 16 u |z|.  Where the codes of z - d and z + d differ (one row in eight at 2816
+// elements; one in forty without y), or a sum of squares leaves the range in which the bounds hold, the CTA takes the
+// row's sums in float64 and redoes the blocks that need it.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "mx.cuh"
+#include "sm100.cuh"
 
 namespace nvfp4b {
 namespace {
 
+enum Src : int { kNone = 0, kBf16 = 1, kF32 = 2 };
+__host__ __device__ constexpr int src_size(Src s) { return s == kF32 ? 4 : s == kBf16 ? 2 : 0; }
+
 constexpr int kNormMaxThreads = 512;
+constexpr int kNormMaxSmem = 220 * 1024;
+constexpr int kRowWarps = 16, kMinRowWarps = 4;          // row kernel: warps per CTA
+constexpr int kRedoList = 512;                           // row kernel: blocks a CTA can leave for its float64 redo
 
 struct NormParams {
     nvfp4b_block_norm_args a;
     int tile_cols;
     float inv_h;
+    int chunks16;        // 8-element chunks, rounded up to the 16 of a scale word
+    int weight_bytes;    // row kernel: shared memory of the weights
+    int in_place;        // an output starts where an input does
+    int stages;          // ring depth, 1 or 2
+    int y_bytes;         // offset of the resid row in a stage
+    int stage_bytes;
+    int gate_vec;        // per-feature gate values may be read 16 bytes at a time
+    int* err;
 };
 
-__device__ __forceinline__ void load8(const void* p, bool f32, long long i, float (&v)[8]) {
-    if (f32) {
-        const float4 q0 = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-        const float4 q1 = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
-        v[0] = q0.x; v[1] = q0.y; v[2] = q0.z; v[3] = q0.w;
-        v[4] = q1.x; v[5] = q1.y; v[6] = q1.z; v[7] = q1.w;
-    } else {
-        const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+// Chunk of 8 values as four pairs.
+struct V8 {
+    float2 p[4];
+    __device__ __forceinline__ float at(int i) const { return (i & 1) ? p[i >> 1].y : p[i >> 1].x; }
+};
+
+__device__ __forceinline__ V8 unpack8(uint4 q) {
+    V8 v;
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { v[2 * j] = bf16lo(w[j]); v[2 * j + 1] = bf16hi(w[j]); }
+    for (int j = 0; j < 4; ++j) v.p[j] = make_float2(bf16lo(w[j]), bf16hi(w[j]));
+    return v;
+}
+
+template <Src S>
+__device__ __forceinline__ V8 load8(const void* row, int ch) {
+    if constexpr (S == kF32) {
+        V8 v;
+        const float4 q0 = static_cast<const float4*>(row)[2 * ch], q1 = static_cast<const float4*>(row)[2 * ch + 1];
+        v.p[0] = make_float2(q0.x, q0.y);
+        v.p[1] = make_float2(q0.z, q0.w);
+        v.p[2] = make_float2(q1.x, q1.y);
+        v.p[3] = make_float2(q1.z, q1.w);
+        return v;
+    } else {
+        return unpack8(static_cast<const uint4*>(row)[ch]);
     }
 }
 
-__device__ __forceinline__ float load1(const void* p, bool f32, long long i) {
-    return f32 ? static_cast<const float*>(p)[i] : __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
+__device__ __forceinline__ V8 fill8(float x) {
+    V8 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v.p[j] = make_float2(x, x);
+    return v;
 }
 
-__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+__device__ __forceinline__ V8 weight8(const void* w, int ch) {
+    return w ? unpack8(__ldg(static_cast<const uint4*>(w) + ch)) : fill8(1.f);
+}
+
+__device__ __forceinline__ uint4 pack8(const V8& v) {
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        const __nv_bfloat162 t = __floats2bfloat162_rn(v.p[j].x, v.p[j].y);
         w[j] = *reinterpret_cast<const uint32_t*>(&t);
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Gate of element (row, i): per token, per feature or per element by its strides; 1 without a gate.
+// Gate of element (row, i): per token, per feature or per element by its strides.
 __device__ __forceinline__ float gate_at(const nvfp4b_block_norm_args& a, int row, int i) {
-    return a.gate ? load1(a.gate, a.gate_f32 != 0, row * a.gate_row_stride + (long long)i * a.gate_col_stride) : 1.0f;
+    const long long o = row * a.gate_row_stride + (long long)i * a.gate_col_stride;
+    return a.gate_f32 ? __ldg(static_cast<const float*>(a.gate) + o)
+                      : __uint_as_float((uint32_t)__ldg(static_cast<const uint16_t*>(a.gate) + o) << 16);
 }
 
-// Block-wide sum, the same bits on every thread.  `red` (one value per warp) must not be in use.
+// Gates of the 8 elements of a chunk (gate_col_stride = 1).
+__device__ __forceinline__ V8 gate8(const NormParams& p, int row, int ch) {
+    const nvfp4b_block_norm_args& a = p.a;
+    if (p.gate_vec) {
+        if (a.gate_f32) return load8<kF32>(static_cast<const float*>(a.gate) + row * a.gate_row_stride, ch);
+        return load8<kBf16>(static_cast<const uint16_t*>(a.gate) + row * a.gate_row_stride, ch);
+    }
+    V8 g;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        g.p[j] = make_float2(gate_at(a, row, ch * 8 + 2 * j), gate_at(a, row, ch * 8 + 2 * j + 1));
+    return g;
+}
+
+__device__ __forceinline__ float sum_sq(const V8& v) {
+    float2 s = __fmul2_rn(v.p[0], v.p[0]);
+#pragma unroll
+    for (int j = 1; j < 4; ++j) s = __ffma2_rn(v.p[j], v.p[j], s);
+    return s.x + s.y;
+}
+
+// Block-wide sums, the same bits on every thread.  `red` must not be in use.
 template <typename T>
 __device__ __forceinline__ T block_sum(T v, T* red) {
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -70,264 +138,838 @@ __device__ __forceinline__ T block_sum(T v, T* red) {
     __syncthreads();
     v = lane < warps ? red[lane] : T(0);
 #pragma unroll
+    for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return __shfl_sync(0xFFFFFFFFu, v, 0);
+}
+
+__device__ __forceinline__ float2 block_sum2(float2 v, float2* red) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        v.x += __shfl_xor_sync(0xFFFFFFFFu, v.x, o);
+        v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, o);
+    }
+    if (lane == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < warps ? red[lane] : make_float2(0.f, 0.f);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) {
+        v.x += __shfl_xor_sync(0xFFFFFFFFu, v.x, o);
+        v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, o);
+    }
+    return make_float2(__shfl_sync(0xFFFFFFFFu, v.x, 0), __shfl_sync(0xFFFFFFFFu, v.y, 0));
+}
+
+template <typename T>
+__device__ __forceinline__ T warp_sum(T v) {
+#pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     return v;
+}
+
+// Sum of squares of a lane's chunks, compensated (each addition's rounding error is kept), and over the warp in float64.
+struct SumSq {
+    float hi = 0.f, lo = 0.f;
+    __device__ __forceinline__ void add(const V8& v) {
+        const float2 q0 = __ffma2_rn(v.p[1], v.p[1], __fmul2_rn(v.p[0], v.p[0]));
+        const float2 q1 = __ffma2_rn(v.p[3], v.p[3], __fmul2_rn(v.p[2], v.p[2]));
+        const float2 q = __fadd2_rn(q0, q1);
+        const float x = q.x + q.y, s = hi + x, b = s - hi;
+        lo += (hi - (s - b)) + (x - b);
+        hi = s;
+    }
+    __device__ __forceinline__ float total() const { return (float)warp_sum((double)hi + (double)lo); }
+};
+
+__device__ __forceinline__ float max_abs(const V8& v) {
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(fabsf(v.p[j].x), fabsf(v.p[j].y)));
+    return m;
+}
+
+__device__ __forceinline__ void store_resid(const nvfp4b_block_norm_args& a, int row, int ch, const V8& r) {
+    if (a.resid_out_f32) {
+        float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.resid_out) + row * a.ld_resid_out) + 2 * ch;
+        o[0] = make_float4(r.p[0].x, r.p[0].y, r.p[1].x, r.p[1].y);
+        o[1] = make_float4(r.p[2].x, r.p[2].y, r.p[3].x, r.p[3].y);
+    } else {
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.resid_out) + row * a.ld_resid_out)[ch] = pack8(r);
+    }
+}
+
+// Returns the largest magnitude (bf16 bits) of the stored values.
+__device__ __forceinline__ uint32_t store_out(const nvfp4b_block_norm_args& a, int row, int ch, const V8& z) {
+    const uint4 q = pack8(z);
+    reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.ld_out)[ch] = q;
+    const uint32_t w = __vmaxu2(__vmaxu2(q.x & 0x7FFF7FFFu, q.y & 0x7FFF7FFFu),
+                                __vmaxu2(q.z & 0x7FFF7FFFu, q.w & 0x7FFF7FFFu));
+    return max(w & 0xFFFFu, w >> 16);
+}
+
+// Padding rows of the last scale tile row, dealt over all threads of the grid.
+__device__ __forceinline__ void zero_padding_rows(const NormParams& p) {
+    const nvfp4b_block_norm_args& a = p.a;
+    const int words = (int)(((long long)a.T + 127) / 128 * 128 - a.T) * p.tile_cols;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < words; i += gridDim.x * blockDim.x)
+        *reinterpret_cast<uint32_t*>(a.scales + mx_scale_offset(a.T + i / p.tile_cols, 4 * (i % p.tile_cols),
+                                                                p.tile_cols)) = 0u;
+}
+
+// The float64 redo of a row: the products of two bf16 values are exact in fp32 (but for overflow and underflow, which
+// only a `wild` row may hold), so those of bf16 sources are converted after the product: the conversions, at an eighth
+// of the fp32 rate, are what the redo costs.
+template <Src S>
+__device__ __forceinline__ double sum_sq64(const V8& v, bool wild) {
+    double q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        q[i] = S == kBf16 && !wild ? (double)(v.at(i) * v.at(i)) : (double)v.at(i) * (double)v.at(i);
+    return ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+}
+
+// r of a chunk in float64; w = the post weights of the chunk, fgs = scale / rms(y), times the gate unless it is per
+// feature.
+template <Src Y, Src R>
+__device__ __forceinline__ void r64(const NormParams& p, int row, int ch, const void* sy, const void* sr, const V8& w,
+                                    double fgs, double (&v)[8], bool wild) {
+    const nvfp4b_block_norm_args& a = p.a;
+    const V8 x = a.resid ? load8<R>(sr, ch) : fill8(0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (double)x.at(i) * (double)a.scale;
+    if constexpr (Y != kNone) {
+        const V8 n = load8<Y>(sy, ch);
+        const bool g_col = a.gate && a.gate_col_stride;
+        const V8 g = g_col ? gate8(p, row, ch) : fill8(1.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double t = Y == kBf16 && !wild ? (double)(n.at(i) * w.at(i)) : (double)n.at(i) * (double)w.at(i);
+            v[i] = fma(g_col ? t * (double)g.at(i) : t, fgs, v[i]);
+        }
+    }
 }
 
 // Whether a mean of squares (+ eps) is in the range where its fp32 value has its relative error bound.
 __device__ __forceinline__ bool mean_ok(float m) { return m > 0x1p-80f && m < 0x1p100f; }
 
-// r of element i in float64; f = 1 / rms(y).
-__device__ __forceinline__ double r64(const nvfp4b_block_norm_args& a, int row, int i, double f) {
-    double r = a.resid ? (double)load1(a.resid, a.resid_f32 != 0, row * a.ld_resid + i) : 0.0;
-    if (a.y) {
-        double n = (double)load1(a.y, a.y_f32 != 0, row * a.ld_y + i) * f;
-        if (a.post_weight) n *= (double)load1(a.post_weight, false, i);
-        r += (double)gate_at(a, row, i) * n;
-    }
-    return r * (double)a.scale;
-}
-
-template <int NCH, bool MX>
-__global__ void __launch_bounds__(kNormMaxThreads) block_norm_kernel(const __grid_constant__ NormParams p) {
-    __shared__ float red[3][kNormMaxThreads / 32];
+template <Src Y, Src R, int NCH, bool MX>
+__global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __grid_constant__ NormParams p) {
+    using namespace sm100;
+    constexpr bool HAS_Y = Y != kNone;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ float red_y[kNormMaxThreads / 32];
+    __shared__ float2 red_r[2][kNormMaxThreads / 32];
     __shared__ double red64[2][kNormMaxThreads / 32];
     __shared__ uint32_t red_max[kNormMaxThreads / 32];
+    __shared__ uint64_t full[2];
+    __shared__ int timeout;
     const nvfp4b_block_norm_args& a = p.a;
-    const int row = blockIdx.x, tid = threadIdx.x, threads = blockDim.x, chunks = a.H >> 3;
-    const bool want_z = a.out || MX;
-    bool redo = false;
+    const int tid = threadIdx.x, threads = blockDim.x, chunks = a.H >> 3;
+    const bool want_z = MX || a.out != nullptr;
 
-    float r[NCH][8], bound[MX ? NCH : 1][8];      // bound: |scale| (|resid| + |gate n|)
-    if (a.y) {
-        float ss = 0.f;
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = tid + c * threads;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) r[c][i] = 0.f;
-            if (ch < chunks) load8(a.y, a.y_f32 != 0, row * a.ld_y + ch * 8, r[c]);
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s = fmaf(r[c][i], r[c][i], s);
-            ss += s;
-        }
-        float f = 1.f;
-        if (a.post_norm) {
-            const float m = fmaf(block_sum(ss, red[0]), p.inv_h, a.eps);
-            redo |= !mean_ok(m);
-            f = __frsqrt_rn(m);
-        }
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = tid + c * threads;
-            if (ch >= chunks) {
-                if constexpr (MX) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) bound[c][i] = 0.f;
-                }
-                continue;
-            }
-            float w[8], v[8], g[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { w[i] = 1.f; v[i] = 0.f; g[i] = 1.f; }
-            if (a.post_weight) load8(a.post_weight, false, ch * 8, w);
-            if (a.resid) load8(a.resid, a.resid_f32 != 0, row * a.ld_resid + ch * 8, v);
-            if (a.gate) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) g[i] = gate_at(a, row, ch * 8 + i);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float t = r[c][i] * f * w[i] * g[i];
-                r[c][i] = a.scale * (v[i] + t);
-                if constexpr (MX) bound[c][i] = fabsf(a.scale) * (fabsf(v[i]) + fabsf(t));
-            }
-        }
-    } else {
-#pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = tid + c * threads;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) r[c][i] = 0.f;
-            if (ch < chunks) load8(a.resid, a.resid_f32 != 0, row * a.ld_resid + ch * 8, r[c]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                r[c][i] *= a.scale;
-                if constexpr (MX) bound[c][i] = fabsf(r[c][i]);
-            }
+    auto fetch = [&](int row, int stage) {              // thread 0: the rows of y and resid into a stage
+        uint8_t* s = ring + stage * p.stage_bytes;
+        const uint32_t yb = (uint32_t)(a.H * src_size(Y)), rb = a.resid ? (uint32_t)(a.H * src_size(R)) : 0u;
+        mbar_arrive_expect_tx(&full[stage], yb + rb);
+        if constexpr (HAS_Y)
+            bulk_load(s, static_cast<const uint8_t*>(a.y) + row * a.ld_y * src_size(Y), yb, &full[stage]);
+        if (rb)
+            bulk_load(s + p.y_bytes, static_cast<const uint8_t*>(a.resid) + row * a.ld_resid * src_size(R), rb,
+                      &full[stage]);
+    };
+    if (tid == 0) {
+        mbar_init(&full[0], 1);
+        mbar_init(&full[1], 1);
+        timeout = 0;
+        fence_mbar_init();
+        for (int s = 0; s < p.stages; ++s) {
+            const long long row = blockIdx.x + (long long)s * gridDim.x;
+            if (row < a.T) fetch((int)row, s);
         }
     }
+    __syncthreads();
 
-    float z[NCH][8];
-    uint32_t code[MX ? NCH : 1], byte[MX ? NCH : 1];
-    if (want_z) {
+    uint32_t zmax = 0, phase = 0;
+    int stage = 0, odd = 0;
+    for (long long lrow = blockIdx.x; lrow < a.T; lrow += gridDim.x) {
+        const int row = (int)lrow;
+        const uint8_t* sy = ring + stage * p.stage_bytes;
+        const uint8_t* sr = sy + p.y_bytes;
+        float2 g_row = make_float2(1.f, 1.f);
+        if (HAS_Y && a.gate && !a.gate_col_stride) g_row.x = g_row.y = gate_at(a, row, 0);
+        mbar_wait(&full[stage], phase, &timeout, kErrTimeoutProducer);   // on expiry the kernel goes on and reports
+
+        V8 r[NCH];
+        float top[NCH];                                  // A of the chunk
         float ss = 0.f, sa = 0.f;
+        bool wild = false;                               // a sum of squares out of range (the same on every thread)
+        float f = 1.f;
+        if constexpr (HAS_Y) {
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            float s = 0.f, t = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s = fmaf(r[c][i], r[c][i], s);
-                if constexpr (MX) t = fmaf(bound[c][i], bound[c][i], t);
+            for (int c = 0; c < NCH; ++c) {
+                const int ch = tid + c * threads;
+                r[c] = ch < chunks ? load8<Y>(sy, ch) : fill8(0.f);
+                ss += sum_sq(r[c]);
             }
-            ss += s;
-            sa += t;
-        }
-        ss = block_sum(ss, red[1]);
-        const float m = fmaf(ss, p.inv_h, a.eps);
-        redo |= !mean_ok(m);
-        const float f = __frsqrt_rn(m);
-        float rel = 0.f;                               // 16 u + 20 u k
-        if constexpr (MX) {
-            if (a.y) {
-                sa = block_sum(sa, red[2]);
-                rel = sa > 0.f ? fmaf(sqrtf(sa / ss), 0x1.4p-20f, 0x1p-20f) : 0.f;
-                redo |= !(rel < 0x1p-10f);             // also where ss = 0 < sa: r cancelled altogether
+            if (a.post_norm) {
+                const float m = fmaf(block_sum(ss, red_y), p.inv_h, a.eps);
+                wild |= !mean_ok(m);
+                f = __frsqrt_rn(m);
             }
-        }
+            const float2 fg = make_float2(f * g_row.x, f * g_row.y), scale = make_float2(a.scale, a.scale);
+            ss = 0.f;
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int ch = tid + c * threads;
-            float w[8];
+            for (int c = 0; c < NCH; ++c) {
+                const int ch = tid + c * threads;
+                top[c] = 0.f;
+                if (ch >= chunks) continue;
+                const V8 w = weight8(a.post_weight, ch);
+                const V8 v = a.resid ? load8<R>(sr, ch) : fill8(0.f);
+                if (a.gate && a.gate_col_stride) {
+                    const V8 g = gate8(p, row, ch);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = 1.f;
-            if (a.norm_weight && ch < chunks) load8(a.norm_weight, false, ch * 8, w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) z[c][i] = ch < chunks ? r[c][i] * f * w[i] : 0.f;
-            if constexpr (MX) {
-                float lo[8], hi[8];
-                uint32_t alo = 0, ahi = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float d = ch >= chunks ? 0.f
-                                    : a.y        ? fabsf(f * w[i]) * fmaf(fabsf(r[c][i]), rel, 0x1.4p-20f * bound[c][i])
-                                                 : 0x1.4p-20f * fabsf(z[c][i]);
-                    lo[i] = z[c][i] - d;
-                    hi[i] = z[c][i] + d;
-                    alo = max(alo, __float_as_uint(fmaxf(fabsf(z[c][i]) - d, 0.f)));
-                    ahi = max(ahi, __float_as_uint(fabsf(z[c][i]) + d) & 0x7FFFFFFFu);
+                    for (int j = 0; j < 4; ++j) r[c].p[j] = __fmul2_rn(r[c].p[j], g.p[j]);
                 }
+                float2 s2 = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    alo = max(alo, __shfl_xor_sync(0xFFFFFFFFu, alo, o));
-                    ahi = max(ahi, __shfl_xor_sync(0xFFFFFFFFu, ahi, o));
+                for (int j = 0; j < 4; ++j) {
+                    const float2 t = __fmul2_rn(r[c].p[j], __fmul2_rn(w.p[j], fg));
+                    r[c].p[j] = __fmul2_rn(__fadd2_rn(v.p[j], t), scale);
+                    if constexpr (MX) {
+                        const float2 b = make_float2(fabsf(v.p[j].x) + fabsf(t.x), fabsf(v.p[j].y) + fabsf(t.y));
+                        top[c] = fmaxf(top[c], fmaxf(b.x, b.y));
+                        s2 = __ffma2_rn(b, b, s2);
+                    }
                 }
-                byte[c] = mx_byte(ahi);
-                const float inv = mx_inv_scale(min(byte[c], 252u));
-                code[c] = mx_encode8(lo, inv);
-                redo |= code[c] != mx_encode8(hi, inv) || byte[c] != mx_byte(alo) || (ahi >> 23) >= 254u ||
-                        (ahi != 0u && ahi < 0x08800000u);     // below 2^-110 the products' bounds fail
+                if constexpr (MX) sa += s2.x + s2.y;
+                if (want_z) ss += sum_sq(r[c]);
+            }
+        } else {
+            const float2 scale = make_float2(a.scale, a.scale);
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const int ch = tid + c * threads;
+                r[c] = ch < chunks ? load8<R>(sr, ch) : fill8(0.f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[c].p[j] = __fmul2_rn(r[c].p[j], scale);
+                ss += sum_sq(r[c]);
             }
         }
-    }
 
-    if (__syncthreads_or(redo)) {                     // the whole row in float64, inputs read again
-        double f = 1.0;
-        if (a.y && a.post_norm) {
+        V8 z[NCH];
+        uint32_t code[NCH], byte[NCH];
+        uint32_t redo = 0;                               // bit c: the block of chunk c is not proven
+        if (want_z) {
+            float rel = 0x1p-20f;                        // 16 u, or 28 u + 16 u k
+            if (MX && HAS_Y) {
+                const float2 s = block_sum2(make_float2(ss, sa), red_r[odd]);
+                ss = s.x;
+                const float k = fabsf(a.scale) * sqrtf(s.y / ss);
+                rel = s.y > 0.f ? fmaf(k, 0x1p-20f, 0x1.cp-20f) : 0.f;
+                wild |= !(rel < 0x1p-12f);               // also where ss = 0 < sa: r cancelled altogether
+            } else {
+                ss = block_sum(ss, reinterpret_cast<float*>(red_r[odd]));
+            }
+            const float m = fmaf(ss, p.inv_h, a.eps);
+            wild |= !mean_ok(m);
+            f = __frsqrt_rn(m);
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const int ch = tid + c * threads;
+                const V8 w = ch < chunks ? weight8(a.norm_weight, ch) : fill8(0.f);
+                const float2 f2 = make_float2(f, f);
+                float zm = 0.f, wm = 0.f;
+                float2 all = make_float2(0.f, 0.f);      // NaN if a z is (a NaN weight passes every maximum)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    z[c].p[j] = __fmul2_rn(r[c].p[j], __fmul2_rn(w.p[j], f2));
+                    if constexpr (MX) all = __fadd2_rn(all, z[c].p[j]);
+                    zm = fmaxf(zm, fmaxf(fabsf(z[c].p[j].x), fabsf(z[c].p[j].y)));
+                    if (MX && HAS_Y) wm = fmaxf(wm, fmaxf(fabsf(w.p[j].x), fabsf(w.p[j].y)));
+                }
+                if constexpr (MX) {
+                    const float d = HAS_Y ? f * fabsf(a.scale) * top[c] * rel : rel;   // per unit of w, or of z
+                    float dm = HAS_Y ? wm * d : zm * rel;
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1) {
+                        zm = fmaxf(zm, __shfl_xor_sync(0xFFFFFFFFu, zm, o));
+                        dm = fmaxf(dm, __shfl_xor_sync(0xFFFFFFFFu, dm, o));
+                    }
+                    const uint32_t top_bits = __float_as_uint(zm + dm);
+                    byte[c] = mx_byte(top_bits);
+                    const float inv = mx_inv_scale(min(byte[c], 252u));
+                    const float2 inv2 = make_float2(inv, inv);
+                    float2 lo[4], hi[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 q = __fmul2_rn(z[c].p[j], inv2), e = HAS_Y ? w.p[j] : q;
+                        const float di = HAS_Y ? d * inv : d;
+                        lo[j] = __ffma2_rn(e, make_float2(-di, -di), q);
+                        hi[j] = __ffma2_rn(e, make_float2(di, di), q);
+                    }
+                    code[c] = cvt_e2m1x8(lo[0].x, lo[0].y, lo[1].x, lo[1].y, lo[2].x, lo[2].y, lo[3].x, lo[3].y);
+                    const uint32_t up = cvt_e2m1x8(hi[0].x, hi[0].y, hi[1].x, hi[1].y, hi[2].x, hi[2].y, hi[3].x, hi[3].y);
+                    const bool doubt = code[c] != up || byte[c] != mx_byte(__float_as_uint(fmaxf(zm - dm, 0.f))) ||
+                                       top_bits >= 0x7F000000u ||
+                                       (top_bits != 0u && top_bits < 0x08800000u) ||  // below 2^-110 no relative bounds
+                                       !(all.x + all.y == all.x + all.y);
+                    redo |= doubt ? 1u << c : 0u;
+                }
+            }
+        }
+        odd ^= 1;
+
+        const bool again = MX ? __syncthreads_or(wild || redo != 0) != 0 : wild;
+        if (again) {                                     // sums of the row in float64; inputs from the stage again
+            double fgs64 = (double)a.scale * (double)g_row.x;
+            if (HAS_Y && a.post_norm) {
+                double s = 0.0;
+#pragma unroll 1
+                for (int ch = tid; ch < chunks; ch += threads) s += sum_sq64<Y>(load8<Y == kF32 ? kF32 : kBf16>(sy, ch), wild);
+                fgs64 *= rsqrt(block_sum(s, red64[0]) / a.H + (double)a.eps);
+            }
             double s = 0.0;
 #pragma unroll 1
-            for (int i = tid; i < a.H; i += threads) {
-                const double v = (double)load1(a.y, a.y_f32 != 0, row * a.ld_y + i);
-                s = fma(v, v, s);
+            for (int ch = tid; ch < chunks; ch += threads) {
+                double v[8];
+                r64<Y, R>(p, row, ch, sy, sr, HAS_Y ? weight8(a.post_weight, ch) : V8(), fgs64, v, wild);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s = fma(v[i], v[i], s);
             }
-            f = 1.0 / sqrt(block_sum(s, red64[0]) / a.H + (double)a.eps);
-        }
-        double s = 0.0;
-#pragma unroll 1
-        for (int i = tid; i < a.H; i += threads) {
-            const double v = r64(a, row, i, f);
-            s = fma(v, v, s);
-        }
-        const double f2 = 1.0 / sqrt(block_sum(s, red64[1]) / a.H + (double)a.eps);
+            const double f2 = rsqrt(block_sum(s, red64[1]) / a.H + (double)a.eps);
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const int ch = tid + c * threads;
+                uint32_t need = wild ? 1u : (redo >> c) & 1u;
+                if constexpr (MX) {                      // the four threads of a block together
+                    need |= __shfl_xor_sync(0xFFFFFFFFu, need, 1);
+                    need |= __shfl_xor_sync(0xFFFFFFFFu, need, 2);
+                }
+                if (!__any_sync(0xFFFFFFFFu, need)) continue;
+                double v[8], amax = 0.0;
+                bool nan = false;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = 0.0;
+                if (need && ch < chunks) {
+                    r64<Y, R>(p, row, ch, sy, sr, HAS_Y ? weight8(a.post_weight, ch) : V8(), fgs64, v, wild);
+                    const V8 w = weight8(a.norm_weight, ch);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const double zz = v[i] * f2 * (double)w.at(i);
+                        if (wild) {
+                            ((i & 1) ? r[c].p[i >> 1].y : r[c].p[i >> 1].x) = (float)v[i];
+                            ((i & 1) ? z[c].p[i >> 1].y : z[c].p[i >> 1].x) = (float)zz;
+                        }
+                        v[i] = zz;
+                        nan |= zz != zz;
+                        amax = fmax(amax, fabs(zz));
+                    }
+                }
+                if constexpr (MX) {
+                    if (nan) amax = __longlong_as_double(0x7FF0000000000000ll);    // as an infinity: byte 0xFF
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1) amax = fmax(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+                    if (need) {
+                        byte[c] = mx_byte64(amax);
+                        code[c] = 0u;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            code[c] |= byte[c] == 255u ? 0u : mx_code64(v[i], byte[c]) << (4 * i);
+                    }
+                }
+            }
+            __syncthreads();                             // every read of the stage before its refill, and of the row
+        }                                                // before the writes (which may be in place)
+        if (!MX && !want_z) __syncthreads();
+        // Everyone has read the stage: the barrier of the last sum, or of the redo, is behind.
+        if (tid == 0 && lrow + (long long)p.stages * gridDim.x < a.T)
+            fetch((int)(lrow + (long long)p.stages * gridDim.x), stage);
+        if (++stage == p.stages) { stage = 0; phase ^= 1u; }
+
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
             const int ch = tid + c * threads;
-            double amax = 0.0;
-            bool nan = false;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (ch >= chunks) continue;
-                const double v = r64(a, row, ch * 8 + i, f);
-                const double w = a.norm_weight ? (double)load1(a.norm_weight, false, ch * 8 + i) : 1.0;
-                const double zz = v * f2 * w;
-                r[c][i] = (float)v;
-                z[c][i] = (float)zz;
-                nan |= zz != zz;
-                amax = fmax(amax, fabs(zz));
-            }
+            const bool ok = ch < chunks;
+            if (a.resid_out && ok) store_resid(a, row, ch, r[c]);
+            if (a.out && ok) zmax = max(zmax, store_out(a, row, ch, z[c]));
             if constexpr (MX) {
-                if (nan) amax = __longlong_as_double(0x7FF0000000000000ll);    // as an infinity: byte 0xFF
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) amax = fmax(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-                byte[c] = mx_byte64(amax);
-                code[c] = 0u;
-#pragma unroll 1
-                for (int i = 0; i < 8; ++i) {
-                    if (ch >= chunks || byte[c] == 255u) continue;
-                    const double v = r64(a, row, ch * 8 + i, f);
-                    const double w = a.norm_weight ? (double)load1(a.norm_weight, false, ch * 8 + i) : 1.0;
-                    code[c] |= mx_code64(v * f2 * w, byte[c]) << (4 * i);
-                }
+                if (ok) reinterpret_cast<uint32_t*>(a.codes + (size_t)row * (a.H >> 1))[ch] = code[c];
+                uint32_t w = ok ? byte[c] << (8 * ((tid & 15) >> 2)) : 0u;
+                w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
+                w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
+                if ((tid & 15) == 0 && (ch >> 4) < p.tile_cols)
+                    *reinterpret_cast<uint32_t*>(a.scales + mx_scale_offset(row, ch >> 2, p.tile_cols)) = w;
             }
         }
-        __syncthreads();                              // every read of the row before the (possibly in-place) writes
     }
 
-    uint32_t zmax = 0;
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-        const int ch = tid + c * threads;
-        const bool ok = ch < chunks;
-        if (a.resid_out && ok) {
-            if (a.resid_out_f32) {
-                float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.resid_out) + row * a.ld_resid_out + ch * 8);
-                o[0] = make_float4(r[c][0], r[c][1], r[c][2], r[c][3]);
-                o[1] = make_float4(r[c][4], r[c][5], r[c][6], r[c][7]);
-            } else {
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.resid_out) + row * a.ld_resid_out + ch * 8) =
-                    pack8(r[c]);
-            }
-        }
-        if (a.out && ok) {
-            const uint4 q = pack8(z[c]);
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.ld_out + ch * 8) = q;
-            const uint32_t w = __vmaxu2(__vmaxu2(q.x & 0x7FFF7FFFu, q.y & 0x7FFF7FFFu),
-                                        __vmaxu2(q.z & 0x7FFF7FFFu, q.w & 0x7FFF7FFFu));
-            zmax = max(zmax, max(w & 0xFFFFu, w >> 16));
-        }
-        if constexpr (MX) {
-            if (ok) *reinterpret_cast<uint32_t*>(a.codes + (size_t)row * (a.H >> 1) + ch * 4) = code[c];
-            uint32_t w = ok ? byte[c] << (8 * ((tid & 15) >> 2)) : 0u;
-            w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
-            w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
-            if ((tid & 15) == 0 && (ch >> 4) < p.tile_cols)
-                *reinterpret_cast<uint32_t*>(a.scales + mx_scale_offset(row, ch >> 2, p.tile_cols)) = w;
-        }
-    }
-    if constexpr (MX) {                               // padding rows of the last scale tile row, dealt over the CTAs
-        const int padded = (a.T + 127) / 128 * 128;
-        for (int m = a.T + row; m < padded; m += gridDim.x)
-            for (int t = tid; t < p.tile_cols; t += threads)
-                *reinterpret_cast<uint32_t*>(a.scales + mx_scale_offset(m, 4 * t, p.tile_cols)) = 0u;
-    }
+    if constexpr (MX) zero_padding_rows(p);
     if (a.amax) {
         zmax = __reduce_max_sync(0xFFFFFFFFu, zmax);
         if ((tid & 31) == 0) red_max[tid >> 5] = zmax;
         __syncthreads();
         if (tid < 32) {
             zmax = __reduce_max_sync(0xFFFFFFFFu, tid < (threads >> 5) ? red_max[tid] : 0u) << 16;
-            // same-address atomics serialise: a row that cannot raise the maximum seen so far skips its own
-            if (tid == 0 && zmax > *reinterpret_cast<volatile uint32_t*>(a.amax))
-                atomicMax(reinterpret_cast<unsigned int*>(a.amax), zmax);
+            if (tid == 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), zmax);
         }
     }
+    if (tid == 0 && timeout != 0) atomicCAS(p.err, 0, timeout);
 }
 
-template <int NCH>
-int launch_block_norm(const NormParams& p, int threads, cudaStream_t s) {
-    return launch_k(p.a.codes ? block_norm_kernel<NCH, true> : block_norm_kernel<NCH, false>, dim3(p.a.T),
-                    dim3(threads), 0, s, p);
+// A row in float64 by a warp.  y and v: the rows of y and resid (valid memory without resid too), in global or shared
+// memory.  A chunk's 24 values are loaded before any is used and no branch parts them: written element by element, each
+// behind its bounds check, a row of 2816 took 32,000 cycles of exposed latencies instead of about 5,000.
+template <Src Y, Src R>
+struct Row64 {
+    const NormParams& p;
+    const void *y, *v;
+    const uint4* w_post;
+    int row, chunks;
+    bool has_v, g_col;
+    double fgs, f, scale;
+
+    __device__ __forceinline__ void r8(int ch, double (&r)[8]) const {
+        const V8 x = load8<R>(v, ch);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) r[k] = has_v ? scale * (double)x.at(k) : 0.0;
+        if constexpr (Y != kNone) {
+            const V8 n = load8<Y>(y, ch), w = unpack8(w_post[ch]);
+            if (g_col) {
+                const V8 g = gate8(p, row, ch);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) r[k] = fma((double)n.at(k) * (double)w.at(k) * (double)g.at(k), fgs, r[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) r[k] = fma((double)n.at(k) * (double)w.at(k), fgs, r[k]);
+            }
+        }
+    }
+    // Sum over the row of the squares of y, or of r.
+    template <bool OF_Y>
+    __device__ __forceinline__ double sum_sq() const {
+        double s = 0.0;
+#pragma unroll 1
+        for (int ch = threadIdx.x & 31; ch < chunks; ch += 32) {
+            double x[8];
+            if constexpr (OF_Y) {
+                const V8 n = load8<Y == kF32 ? kF32 : kBf16>(y, ch);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = (double)n.at(k);
+            } else {
+                r8(ch, x);
+            }
+            s += fma(x[0], x[0], x[1] * x[1]) + fma(x[2], x[2], x[3] * x[3]) +
+                 (fma(x[4], x[4], x[5] * x[5]) + fma(x[6], x[6], x[7] * x[7]));
+        }
+        return warp_sum(s);
+    }
+    __device__ __forceinline__ Row64(const NormParams& p_, int row_, const void* y_, const void* v_, const uint4* w_post_)
+        : p(p_), y(y_), v(v_), w_post(w_post_), row(row_), chunks(p_.a.H >> 3), has_v(p_.a.resid != nullptr),
+          scale((double)p_.a.scale) {
+        const double h = (double)p.a.H, eps = (double)p.a.eps;
+        g_col = Y != kNone && p.a.gate && p.a.gate_col_stride;
+        fgs = scale * (Y != kNone && p.a.gate && !g_col ? (double)gate_at(p.a, row, 0) : 1.0);
+        if (Y != kNone && p.a.post_norm) fgs *= rsqrt(sum_sq<true>() / h + eps);
+        f = rsqrt(sum_sq<false>() / h + eps);
+    }
+};
+
+// The codes and scales of the loop steps (32 chunks each) in `steps`, or for a `wild` row everything (both the same on
+// every lane).  Returns the largest bf16 magnitude stored to out.
+template <Src Y, Src R, bool MX>
+__device__ __noinline__ uint32_t redo_row64(const NormParams& p, int row, uint32_t steps, bool wild, const void* y,
+                                            const void* v, const uint4* w_post, const uint4* w_norm) {
+    const nvfp4b_block_norm_args& a = p.a;
+    const int lane = threadIdx.x & 31;
+    const Row64<Y, R> q(p, row, y, v, w_post);
+    __syncwarp();                                                   // codes and scale words stored before come first
+    uint32_t zmax = 0;
+    int step = 0;
+#pragma unroll 1
+    for (int c0 = 0; c0 < p.chunks16; c0 += 32, ++step) {
+        if (!wild && !((steps >> step) & 1u)) continue;
+        const int ch = c0 + lane;
+        const bool ok = ch < q.chunks;
+        double z[8], amax = 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) z[k] = 0.0;
+        if (ok) {
+            q.r8(ch, z);
+            const V8 w = unpack8(w_norm[ch]);
+            V8 s;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s.p[j] = make_float2((float)z[2 * j], (float)z[2 * j + 1]);
+            if (wild && a.resid_out) store_resid(a, row, ch, s);    // in place: the lane has read its own chunk
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                z[k] = z[k] * q.f * (double)w.at(k);
+                amax = z[k] != z[k] ? __longlong_as_double(0x7FF0000000000000ll) : fmax(amax, fabs(z[k]));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s.p[j] = make_float2((float)z[2 * j], (float)z[2 * j + 1]);
+            if (wild && a.out) zmax = max(zmax, store_out(a, row, ch, s));
+        }
+        if constexpr (MX) {
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) amax = fmax(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+            const uint32_t byte = mx_byte64(amax);                  // NaN came as an infinity: byte 0xFF
+            uint32_t code = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) code |= byte == 255u ? 0u : mx_code64(z[k], byte) << (4 * k);
+            if (ok) reinterpret_cast<uint32_t*>(a.codes + (size_t)row * (a.H >> 1))[ch] = code;
+            if ((lane & 3) == 0 && ch < p.chunks16)
+                a.scales[mx_scale_offset(row, ch >> 2, p.tile_cols)] = ok ? (uint8_t)byte : (uint8_t)0;
+        }
+    }
+    return zmax;
+}
+
+// Many rows: a row per warp.  No block-wide barrier, and the fixed cost of a row (two reductions, the wait for its bulk
+// copies) is paid by one warp instead of all warps of a CTA.  Each warp owns one row buffer in shared memory; the weights
+// lie there once per CTA; the next row is prefetched into L2 meanwhile.  Pass 1: sum of y^2.  Pass 2: r, written over
+// the chunk's own y and resid, and the sums of r^2 and t^2 (t = scale * gate * n).  Pass 3: outputs.  Short code at any
+// H, and 16 warps per SM hide each other's latencies (two stages and 8 warps: 92 against 70 us at 8192 x 2816).
+//
+// Bounds: a chunk's sum of squares is off by 4 u of itself, its compensated sum over the row's chunks and the float64
+// tree by less than 0.1 u more, 1 / rms by 4.5 u; t by 8.5 u |t|, r by that + u |r|, and z (the rounding of z - d and
+// z + d included) by
+//   d = f wm E T + Z E (1 + k),   E = 10 u,   k = sqrt(sum t^2 / sum r^2),   wm = max |norm_w|,
+// T = max |t| of the lane's chunks, Z = max |z| of the chunk (one d serves its 8 elements); without y by E |z|.  One row
+// in sixteen at 2816 elements holds an element that near to a border.  Those rows are listed and redone at the end, one
+// per warp at a time: redone on the spot, a row's float64 latency lands on one warp of the SM (76 against 51 us without
+// any redo).
+template <Src Y, Src R, bool MX>
+__global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(const __grid_constant__ NormParams p) {
+    using namespace sm100;
+    constexpr bool HAS_Y = Y != kNone;
+    constexpr float kE = 0x1.4p-21f;                                // 10 u
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t full[kRowWarps];
+    __shared__ uint32_t red_max[kRowWarps];
+    __shared__ int2 redo_list[kRedoList];                           // row, unproven block
+    __shared__ int listed, timeout;
+    const nvfp4b_block_norm_args& a = p.a;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5, chunks = a.H >> 3;
+    const bool want_z = MX || a.out != nullptr;
+    uint4* w_post = reinterpret_cast<uint4*>(smem);                 // bf16, ones where there are none
+    uint4* w_norm = w_post + (HAS_Y ? chunks : 0);
+    uint8_t* const sy = smem + p.weight_bytes + wid * p.stage_bytes;
+    uint8_t* const sr = sy + p.y_bytes;
+    // r of a chunk takes the place of its inputs: 32 bytes of the fp32 one, or 16 of either bf16 one
+    auto r_lo = [&](int ch) { return reinterpret_cast<float4*>(Y == kF32 ? sy + 32 * ch : R == kF32 ? sr + 32 * ch : sy + 16 * ch); };
+    auto r_hi = [&](int ch) { return reinterpret_cast<float4*>(Y == kF32 ? sy + 32 * ch + 16 : R == kF32 ? sr + 32 * ch + 16 : sr + 16 * ch); };
+
+    const uint32_t yb = (uint32_t)(a.H * src_size(Y)), rb = a.resid ? (uint32_t)(a.H * src_size(R)) : 0u;
+    auto y_row = [&](long long row) { return static_cast<const uint8_t*>(a.y) + row * a.ld_y * src_size(Y); };
+    auto v_row = [&](long long row) { return static_cast<const uint8_t*>(a.resid) + row * a.ld_resid * src_size(R); };
+    auto fetch = [&](long long row) {                               // lane 0
+        mbar_arrive_expect_tx(&full[wid], yb + rb);
+        if constexpr (HAS_Y) bulk_load(sy, y_row(row), yb, &full[wid]);
+        if (rb) bulk_load(sr, v_row(row), rb, &full[wid]);
+    };
+    const long long first = (long long)blockIdx.x * warps + wid, step = (long long)gridDim.x * warps;
+    if (threadIdx.x == 0) timeout = listed = 0;
+    if (lane == 0) {
+        mbar_init(&full[wid], 1);
+        fence_mbar_init();
+        if (first < a.T) fetch(first);
+    }
+    const uint4 ones = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);
+    uint32_t wm_bits = 0;
+    for (int ch = threadIdx.x; ch < chunks; ch += blockDim.x) {
+        if (HAS_Y) w_post[ch] = a.post_weight ? static_cast<const uint4*>(a.post_weight)[ch] : ones;
+        const uint4 q = a.norm_weight ? static_cast<const uint4*>(a.norm_weight)[ch] : ones;
+        w_norm[ch] = q;
+        const uint32_t m = __vmaxu2(__vmaxu2(q.x & 0x7FFF7FFFu, q.y & 0x7FFF7FFFu),
+                                    __vmaxu2(q.z & 0x7FFF7FFFu, q.w & 0x7FFF7FFFu));
+        wm_bits = max(wm_bits, max(m & 0xFFFFu, m >> 16));
+    }
+    wm_bits = __reduce_max_sync(0xFFFFFFFFu, wm_bits);
+    if (lane == 0) red_max[wid] = wm_bits;
+    __syncthreads();
+    const float wm = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, lane < warps ? red_max[lane] : 0u) << 16);
+    __syncthreads();                                                // red_max is used again at the end
+
+    uint32_t zmax = 0, phase = 0;
+    for (long long lrow = first; lrow < a.T; lrow += step) {
+        const int row = (int)lrow;
+        const float g_row = HAS_Y && a.gate && !a.gate_col_stride ? gate_at(a, row, 0) : 1.f;
+        const bool g_col = HAS_Y && a.gate && a.gate_col_stride;
+        mbar_wait(&full[wid], phase, &timeout, kErrTimeoutProducer);   // on expiry the kernel goes on and reports
+        phase ^= 1u;
+        if (lane == 0 && lrow + step < a.T) {
+            if constexpr (HAS_Y) l2_prefetch(y_row(lrow + step), yb);
+            if (rb) l2_prefetch(v_row(lrow + step), rb);
+        }
+        bool wild = false;
+        float fgs = 1.f;                                            // scale * gate / rms(y)
+        if constexpr (HAS_Y) {
+            float f = 1.f;
+            if (a.post_norm) {
+                SumSq ss;
+#pragma unroll 4
+                for (int ch = lane; ch < chunks; ch += 32) ss.add(load8<Y>(sy, ch));
+                const float m = fmaf(ss.total(), p.inv_h, a.eps);
+                wild |= !mean_ok(m);
+                f = __frsqrt_rn(m);
+            }
+            fgs = f * g_row * a.scale;
+        }
+        const float2 scale2 = make_float2(a.scale, a.scale);
+        float t_max = 0.f, st = 0.f;
+        SumSq ss;
+        if constexpr (HAS_Y) {
+            const float2 fgs2 = make_float2(fgs, fgs);
+#pragma unroll 2
+            for (int ch = lane; ch < chunks; ch += 32) {
+                const V8 y = load8<Y>(sy, ch), w = unpack8(w_post[ch]), v = a.resid ? load8<R>(sr, ch) : fill8(0.f);
+                V8 t, r;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) t.p[j] = __fmul2_rn(y.p[j], __fmul2_rn(w.p[j], fgs2));
+                if (g_col) {
+                    const V8 g = gate8(p, row, ch);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t.p[j] = __fmul2_rn(t.p[j], g.p[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r.p[j] = __ffma2_rn(v.p[j], scale2, t.p[j]);
+                *r_lo(ch) = make_float4(r.p[0].x, r.p[0].y, r.p[1].x, r.p[1].y);
+                *r_hi(ch) = make_float4(r.p[2].x, r.p[2].y, r.p[3].x, r.p[3].y);
+                ss.add(r);
+                if constexpr (MX) {
+                    st += sum_sq(t);
+                    t_max = fmaxf(t_max, max_abs(t));
+                }
+            }
+        } else {
+#pragma unroll 4
+            for (int ch = lane; ch < chunks; ch += 32) {
+                V8 v = load8<R>(sr, ch);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v.p[j] = __fmul2_rn(v.p[j], scale2);
+                ss.add(v);
+            }
+        }
+        auto r_chunk = [&](int ch) {
+            V8 r;
+            if constexpr (HAS_Y) {
+                const float4 q0 = *r_lo(ch), q1 = *r_hi(ch);
+                r.p[0] = make_float2(q0.x, q0.y);
+                r.p[1] = make_float2(q0.z, q0.w);
+                r.p[2] = make_float2(q1.x, q1.y);
+                r.p[3] = make_float2(q1.z, q1.w);
+            } else {
+                r = load8<R>(sr, ch);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r.p[j] = __fmul2_rn(r.p[j], scale2);
+            }
+            return r;
+        };
+        float f = 1.f, rel = kE;
+        if (want_z) {
+            const float sum = ss.total();
+            if constexpr (MX && HAS_Y) {
+                st = warp_sum(st);
+                rel = st > 0.f ? fmaf(sqrtf(st / sum), kE, kE) : kE;
+                wild |= !(rel < 0x1p-12f);                          // also where sum = 0 < st: r cancelled altogether
+            }
+            const float m = fmaf(sum, p.inv_h, a.eps);
+            wild |= !mean_ok(m) || (MX && !(wm < __int_as_float(0x7F800000)));   // a NaN weight passes every maximum
+            f = __frsqrt_rn(m);
+        }
+        const float2 f2 = make_float2(f, f);
+        auto z_chunk = [&](int ch, const V8& r) {
+            const V8 w = unpack8(w_norm[ch]);
+            V8 z;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z.p[j] = __fmul2_rn(r.p[j], __fmul2_rn(w.p[j], f2));
+            return z;
+        };
+        uint32_t row_max = 0, doubt = 0;                            // bit i: the chunk of loop step i is not proven
+        // r and z are stored at once, unless that would overwrite what a redo reads again
+        const bool later = MX && p.in_place;
+        if (!wild) {
+            const float dt = t_max * f * wm * kE;
+            uint32_t* code_row = reinterpret_cast<uint32_t*>(a.codes + (MX ? (size_t)row * (a.H >> 1) : 0));
+            uint8_t* scale_row = a.scales + (MX ? mx_scale_offset(row, 0, p.tile_cols) : 0);   // + 512 per 16 chunks
+            int i = 0;
+#pragma unroll 1
+            for (int c0 = 0; c0 < p.chunks16; c0 += 32, ++i) {      // whole groups of 16: the scale words' threads
+                const int ch = c0 + lane;
+                const bool ok = ch < chunks;
+                V8 z;
+                if (ok) {
+                    const V8 r = r_chunk(ch);
+                    if (a.resid_out && !later) store_resid(a, row, ch, r);
+                    z = z_chunk(ch, r);
+                    if (a.out && !later) row_max = max(row_max, store_out(a, row, ch, z));
+                } else {
+                    z = fill8(0.f);
+                }
+                if constexpr (MX) {
+                    float zm = max_abs(z);
+                    const float d = HAS_Y && ok ? fmaf(zm, rel, dt) : zm * rel;
+                    float dm = d;
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1) {
+                        zm = fmaxf(zm, __shfl_xor_sync(0xFFFFFFFFu, zm, o));
+                        dm = fmaxf(dm, __shfl_xor_sync(0xFFFFFFFFu, dm, o));
+                    }
+                    const uint32_t top = __float_as_uint(zm + dm), bot = __float_as_uint(fmaxf(zm - dm, 0.f));
+                    // exponent field, at least 2; the byte is 2 less, and 1 / 2^e has the field 256 - it
+                    const uint32_t field = max(top & 0x7F800000u, 0x01000000u);
+                    const float inv = __uint_as_float(0x80000000u - field);
+                    const float2 inv2 = make_float2(inv, inv);
+                    // without y the bound is relative to each element
+                    const float2 up = HAS_Y ? make_float2(d * inv, d * inv) : make_float2(rel, rel);
+                    const float2 dn = make_float2(-up.x, -up.y);
+                    float2 lo[4], hi[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 q = __fmul2_rn(z.p[j], inv2);
+                        lo[j] = HAS_Y ? __fadd2_rn(q, dn) : __ffma2_rn(q, dn, q);
+                        hi[j] = HAS_Y ? __fadd2_rn(q, up) : __ffma2_rn(q, up, q);
+                    }
+                    const uint32_t code =
+                        cvt_e2m1x8(lo[0].x, lo[0].y, lo[1].x, lo[1].y, lo[2].x, lo[2].y, lo[3].x, lo[3].y);
+                    const uint32_t other =
+                        cvt_e2m1x8(hi[0].x, hi[0].y, hi[1].x, hi[1].y, hi[2].x, hi[2].y, hi[3].x, hi[3].y);
+                    // also where the exponent is in doubt, or the values are near the ends of the range
+                    const bool unsure = code != other || ((top ^ bot) & 0x7F800000u) != 0u ||
+                                        top - 0x08800000u >= 0x7F000000u - 0x08800000u;
+                    if (unsure && top != 0u) {
+                        int slot = kRedoList;
+                        if (!later) slot = atomicAdd(&listed, 1);    // a block may be listed by each of its four lanes
+                        if (slot < kRedoList) redo_list[slot] = make_int2(row, ch >> 2);
+                        else doubt |= 1u << i;
+                    }
+                    if (ok) code_row[ch] = code;
+                    uint32_t w = ok ? ((field >> 23) - 2u) << (8 * ((lane & 15) >> 2)) : 0u;
+                    w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
+                    w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
+                    if ((lane & 15) == 0 && ch < p.chunks16) *reinterpret_cast<uint32_t*>(scale_row + 32 * ch) = w;
+                }
+            }
+        }
+        doubt = __reduce_or_sync(0xFFFFFFFFu, doubt);               // from here on the same on every lane, as `wild` is
+        if (wild || doubt != 0) {
+            const uint32_t m = redo_row64<Y, R, MX>(p, row, doubt, wild, y_row(row), a.resid ? v_row(row) : smem, w_post, w_norm);
+            row_max = wild ? m : row_max;
+        }
+        if (later && !wild) {
+#pragma unroll 1
+            for (int ch = lane; ch < chunks; ch += 32) {
+                const V8 r = r_chunk(ch);
+                if (a.resid_out) store_resid(a, row, ch, r);
+                if (a.out) row_max = max(row_max, store_out(a, row, ch, z_chunk(ch, r)));
+            }
+        }
+        zmax = max(zmax, row_max);
+        fence_proxy_async();                                        // r's writes before the copies' ones
+        __syncwarp();                                               // every lane is done with the buffer
+        if (lane == 0 && lrow + step < a.T) fetch(lrow + step);
+    }
+
+    if constexpr (MX) {
+        zero_padding_rows(p);
+        __syncthreads();
+        for (int i = wid; i < min(listed, kRedoList); i += warps) {
+            const int2 e = redo_list[i];
+            if (lane == 0) fetch(e.x);
+            mbar_wait(&full[wid], phase, &timeout, kErrTimeoutProducer);
+            phase ^= 1u;
+            redo_row64<Y, R, true>(p, e.x, 1u << (e.y >> 3), false, sy, sr, w_post, w_norm);
+            __syncwarp();                                           // every lane is done with the buffer
+        }
+    }
+    if (a.amax) {
+        zmax = __reduce_max_sync(0xFFFFFFFFu, zmax);
+        if (lane == 0) red_max[wid] = zmax;
+        __syncthreads();
+        if (wid == 0) {
+            zmax = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? red_max[lane] : 0u) << 16;
+            if (lane == 0) atomicMax(reinterpret_cast<unsigned int*>(a.amax), zmax);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && timeout != 0) atomicCAS(p.err, 0, timeout);
+}
+
+int raise_smem(const void* kernel, std::atomic<bool> (&ready)[64]) {   // once per kernel and device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NVFP4B_ERR_CUDA;
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kNormMaxSmem);
+        if (e != cudaSuccess) return record_cuda_error(e);
+        ready[dev].store(true, std::memory_order_release);
+    }
+    return NVFP4B_OK;
+}
+
+// The row kernel's launch; `fits` false (nothing launched) where shared memory holds fewer than kMinRowWarps row buffers
+// or a row has more loop steps than a 32-bit mask.
+template <Src Y, Src R, bool MX>
+int launch_block_norm_rows(NormParams& p, cudaStream_t s, bool& fits) {
+    const auto kernel = block_norm_rows_kernel<Y, R, MX>;
+    p.y_bytes = p.a.H * src_size(Y);
+    p.stage_bytes = (p.a.H * (src_size(Y) + src_size(R)) + 127) / 128 * 128;
+    p.weight_bytes = (p.a.H * (Y == kNone ? 2 : 4) + 127) / 128 * 128;
+    int warps = (kNormMaxSmem - p.weight_bytes) / p.stage_bytes;
+    fits = warps >= kMinRowWarps && p.a.H <= 32 * 256;
+    if (!fits) return NVFP4B_OK;
+    if (warps > kRowWarps) warps = kRowWarps;
+    // the count of warps whose last round of rows leaves the fewest idle
+    const int sms = sm_count();
+    long long best = -1;
+    for (int w = warps, most = warps; w >= most - most / 4; --w) {
+        const long long rounds = (p.a.T + (long long)sms * w - 1) / ((long long)sms * w) * w;
+        if (best < 0 || rounds < best) { best = rounds; warps = w; }
+    }
+    static std::atomic<bool> ready[64];
+    const int st = raise_smem(reinterpret_cast<const void*>(kernel), ready);
+    if (st) return st;
+    long long grid = ((long long)p.a.T + warps - 1) / warps;
+    if (grid > sms) grid = sms;
+    return launch_k(kernel, dim3((unsigned)grid), dim3(warps * 32), p.weight_bytes + warps * p.stage_bytes, s, p);
+}
+
+// Persistent grid: as many CTAs per SM as shared memory (and 2048 threads at up to 128 registers) hold.
+template <Src Y, Src R, int NCH, bool MX>
+int launch_block_norm(NormParams& p, cudaStream_t s) {
+    const auto kernel = block_norm_kernel<Y, R, NCH, MX>;
+    static std::atomic<bool> ready[64];
+    const int st = raise_smem(reinterpret_cast<const void*>(kernel), ready);
+    if (st) return st;
+    const int threads = (p.a.H / 8 + NCH * 32 - 1) / (NCH * 32) * 32;
+    const int row_bytes = p.a.H * src_size(Y) + (p.a.resid ? p.a.H * src_size(R) : 0);
+    p.y_bytes = p.a.H * src_size(Y);                     // a multiple of 16
+    p.stage_bytes = (row_bytes + 127) / 128 * 128;
+    p.stages = 2 * p.stage_bytes <= kNormMaxSmem ? 2 : 1;
+    const int smem = p.stages * p.stage_bytes;
+    int per_sm = kNormMaxSmem / (smem + 1024);
+    const int by_regs = 512 / threads;
+    if (per_sm > by_regs) per_sm = by_regs;
+    if (per_sm < 1) per_sm = 1;
+    long long grid = (long long)sm_count() * per_sm;
+    if (grid > p.a.T) grid = p.a.T;
+    return launch_k(kernel, dim3((unsigned)grid), dim3(threads), smem, s, p);
+}
+
+// A CTA per row, one chunk per thread where that fits (four above 4096 elements); from kRowKernelRows rows per SM on, a
+// warp per row, where its rings fit (rows of up to 24 KB of input).
+constexpr int kRowKernelRows = 8;
+
+template <Src Y, Src R>
+int dispatch_block_norm(NormParams& p, cudaStream_t s) {   // R = kBf16 without resid
+    if (p.a.T >= kRowKernelRows * sm_count()) {
+        bool fits = false;
+        const int st = p.a.codes ? launch_block_norm_rows<Y, R, true>(p, s, fits)
+                                 : launch_block_norm_rows<Y, R, false>(p, s, fits);
+        if (fits) return st;
+    }
+    const bool wide = p.a.H <= 8 * kNormMaxThreads;
+    if (p.a.codes) return wide ? launch_block_norm<Y, R, 1, true>(p, s) : launch_block_norm<Y, R, 4, true>(p, s);
+    return wide ? launch_block_norm<Y, R, 1, false>(p, s) : launch_block_norm<Y, R, 4, false>(p, s);
 }
 
 bool bad_rows(const void* p, int f32, long long ld) { return !aligned16(p) || (ld * (f32 ? 4 : 2)) % 16; }
@@ -367,9 +1009,16 @@ extern "C" int nvfp4b_block_norm(const nvfp4b_block_norm_args* args, void* strea
     p.a = a;
     p.tile_cols = (a.H + 127) / 128;
     p.inv_h = 1.0f / (float)a.H;
-    const int chunks = a.H / 8, nch = chunks <= kNormMaxThreads ? 1 : chunks <= 2 * kNormMaxThreads ? 2 : 4;
-    const int threads = (chunks + nch * 32 - 1) / (nch * 32) * 32;
-    if (nch == 1) return launch_block_norm<1>(p, threads, s);
-    if (nch == 2) return launch_block_norm<2>(p, threads, s);
-    return launch_block_norm<4>(p, threads, s);
+    p.chunks16 = p.tile_cols * 16;
+    p.weight_bytes = 0;
+    p.in_place = (a.resid_out && (a.resid_out == a.resid || a.resid_out == a.y)) ||
+                 (a.out && (a.out == a.resid || a.out == a.y));
+    p.gate_vec = aligned16(a.gate) && (a.gate_row_stride * (a.gate_f32 ? 4 : 2)) % 16 == 0;
+    p.err = device_error_ptr();
+    if (!p.err) return NVFP4B_ERR_CUDA;
+    const bool f32 = a.resid && a.resid_f32;
+    if (a.y && a.y_f32)
+        return f32 ? dispatch_block_norm<kF32, kF32>(p, s) : dispatch_block_norm<kF32, kBf16>(p, s);
+    if (a.y) return f32 ? dispatch_block_norm<kBf16, kF32>(p, s) : dispatch_block_norm<kBf16, kBf16>(p, s);
+    return f32 ? dispatch_block_norm<kNone, kF32>(p, s) : dispatch_block_norm<kNone, kBf16>(p, s);
 }

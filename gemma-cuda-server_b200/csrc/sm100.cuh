@@ -117,6 +117,17 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
         : "memory");
 }
 
+// Prefetch `bytes` (a multiple of 16, 16-byte aligned) of global memory into L2.
+__device__ __forceinline__ void l2_prefetch(const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(src)), "r"(bytes)
+                 : "memory");
+}
+
+// Orders this thread's (and, behind a barrier, its peers') shared-memory writes before later async-proxy accesses.
+__device__ __forceinline__ void fence_proxy_async() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
 // L2 eviction priority for data read once (a streamed operand): first in line for eviction, so the hot working set
 // (activations, the row buffers a following kernel reads back) stays in L2 while the stream passes through.
 __device__ __forceinline__ uint64_t l2_policy_evict_first() {

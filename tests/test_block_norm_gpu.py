@@ -86,7 +86,7 @@ B, F = torch.bfloat16, torch.float32
 
 
 @pytest.mark.parametrize("T,H", [(1, 32), (1, 2816), (3, 96), (130, 160), (129, 2816), (64, 4096), (9, 4128), (5, 8224),
-                                 (2, 16384), (300, 2112)])
+                                 (2, 16384), (300, 2112), (1190, 160), (1203, 2112), (1185, 544), (1, 12288)])
 @pytest.mark.parametrize("resid,y", [(B, None), (F, None), (B, B), (F, F), (B, F), (None, B)])
 def test_norm_to_mxfp4_and_bf16(T, H, resid, y):
     p = require_gpu()
@@ -96,20 +96,24 @@ def test_norm_to_mxfp4_and_bf16(T, H, resid, y):
     _check(p, T, H, False, True, scale=-1.7, eps=1e-5, **kw)
 
 
-@pytest.mark.parametrize("T,H", [(1, 8), (5, 24), (33, 1000), (2, 5000)])
+@pytest.mark.parametrize("T,H", [(1, 8), (5, 24), (33, 1000), (2, 5000), (1300, 8), (1200, 1000)])
 def test_widths_of_a_multiple_of_eight(T, H):
     p = require_gpu()
     _check(p, T, H, False, True, **_make(T, H, H, F, B, gate="row"))
 
 
 @pytest.mark.parametrize("gate,dtype", list(itertools.product(["feature", "row", "full"], [B, F])))
-def test_gates(gate, dtype):
+@pytest.mark.parametrize("T", [70, 1200])
+def test_gates(T, gate, dtype):
     p = require_gpu()
-    kw = _make(70, 704, 5, B, B, gate=gate)
+    kw = _make(T, 704, 5, B, B, gate=gate)
     kw["gate"] = kw["gate"].to(dtype)
-    _check(p, 70, 704, True, True, scale=0.5, **kw)
-    kw["gate"] = torch.cat([kw["gate"], kw["gate"]], -1)[..., :kw["gate"].shape[-1]]          # strided
-    _check(p, 70, 704, True, True, scale=0.5, **kw)
+    _check(p, T, 704, True, True, scale=0.5, **kw)
+    n = kw["gate"].shape[-1]
+    kw["gate"] = torch.cat([kw["gate"], kw["gate"]], -1)[..., :n]                             # strided rows
+    _check(p, T, 704, True, True, scale=0.5, **kw)
+    kw["gate"] = torch.cat([kw["gate"][..., :1], kw["gate"]], -1)[..., 1:]                    # no wide loads
+    _check(p, T, 704, True, True, scale=0.5, **kw)
 
 
 @pytest.mark.parametrize("post_norm", [True, False])
@@ -129,13 +133,15 @@ def test_many_rows_equal_codes():
         _check(p, 2000, 2816, True, False, **_make(2000, 2816, 11, resid, y, gate=gate))
 
 
-def test_rows_that_cancel_vanish_or_overflow():
+@pytest.mark.parametrize("T", [12, 1300])
+@pytest.mark.parametrize("dtype", [B, F])
+def test_rows_that_cancel_vanish_or_overflow(T, dtype):
     """resid = -n up to rounding, zero rows, subnormal and huge rows, NaN and infinities: the float64 codes all the same."""
     p = require_gpu()
-    T, H = 12, 160
-    kw = _make(T, H, 8, F, F)
+    H = 160
+    kw = _make(T, H, 8, dtype, dtype)
     r, _ = mx.block_norm(None, None, float(np.float32(1e-6)), _n(kw["y"]), _n(kw["post_weight"]))
-    kw["resid"][:4] = torch.from_numpy(-r[:4]).float().cuda()
+    kw["resid"][:4] = torch.from_numpy(-r[:4]).to(dtype).cuda()
     kw["resid"][4], kw["y"][4] = 0, 0
     kw["resid"][5] *= 1e-40
     kw["y"][5] *= 1e-42
@@ -143,7 +149,7 @@ def test_rows_that_cancel_vanish_or_overflow():
     kw["y"][7] *= 1e25
     kw["resid"][8, 3], kw["y"][9, 5], kw["resid"][10, 0] = float("nan"), float("inf"), float("-inf")
     kw["y"][11] = 0
-    r, z, _, _ = _want(kw)
+    r, z, dr, dz = _want(kw)
     codes, scales = poisoned(T * H // 2).view(T, H // 2), poisoned(mx.scale_buffer_bytes(T, H))
     out = torch.empty(T, H, dtype=B, device="cuda")
     p.block_norm(codes=codes, scales=scales, out=out, resid_out=kw["resid"], **kw)            # in place
@@ -151,8 +157,30 @@ def test_rows_that_cancel_vanish_or_overflow():
     byte, clean = mx.untile_scales(scales.cpu().numpy(), T, H)
     assert np.array_equal(byte, ref[1]) and clean and np.array_equal(codes.cpu().numpy(), ref[0])
     assert np.array_equal(np.isnan(_n(out)), np.isnan(z))
-    ok = np.isfinite(z)
-    assert (np.abs(_n(out)[ok] - z[ok]) <= np.abs(z[ok]) * 2.0 ** -7).all()
+    whole = np.isfinite(r).all(1)                              # the other rows: infinities, and x / inf = 0, or NaN
+    _near(out[torch.from_numpy(whole)], z[whole], dz[whole], B)
+    _near(kw["resid"][torch.from_numpy(whole)], r[whole], dr[whole], dtype)
+    assert np.array_equal(_n(out)[~whole], z[~whole], equal_nan=True)
+
+
+@pytest.mark.parametrize("T", [12, 1300])
+def test_weights_that_are_not_finite(T):
+    """A NaN or infinite weight of the second norm spoils exactly its block of every row."""
+    p = require_gpu()
+    for kind in (None, B):
+        kw = _make(T, 160, 13, B, kind)
+        clean = p.block_norm(mx=True, **kw)
+        for bad in (float("nan"), float("inf")):
+            kw["norm_weight"][70] = bad
+            got = p.block_norm(mx=True, **kw)
+            byte, _ = mx.untile_scales(got.scales.cpu().numpy(), T, 160)
+            want, _ = mx.untile_scales(clean.scales.cpu().numpy(), T, 160)
+            want[:, 2] = 255
+            assert np.array_equal(byte, want)
+            keep = [i for i in range(80) if not 32 <= i < 48]
+            assert torch.equal(got.codes[:, keep], clean.codes[:, keep]) and not got.codes[:, 32:48].any()
+            kw["norm_weight"][70] = 1.0
+            clean = p.block_norm(mx=True, **kw)
 
 
 def test_zero_eps_and_zero_rows():
