@@ -275,32 +275,36 @@ def _mx_sigs():
     return L
 
 
-def _rows(name: str, t: torch.Tensor, dtypes, shape, device=None) -> int:
+def _rows(name: str, t: torch.Tensor, dtypes, shape, device: int | None = None) -> int:
     """Checks a [rows, columns] CUDA tensor with unit column stride; returns its row pitch in elements.  None in
-    `shape` stands for any size."""
+    `shape` stands for any size, None for the device index for any CUDA device."""
+    got = t.shape
     if t.dtype not in dtypes:
         raise ValueError(f"{name}: dtype {t.dtype}, expected one of {dtypes}")
-    if t.dim() != 2 or any(w is not None and w != g for w, g in zip(shape, t.shape)):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if not t.is_cuda or (device is not None and t.device != device):
-        raise ValueError(f"{name}: on {t.device}, expected {device or 'a CUDA device'}")
-    rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    if len(got) != 2 or (shape[0] is not None and shape[0] != got[0]) or (shape[1] is not None and shape[1] != got[1]):
+        raise ValueError(f"{name}: shape {tuple(got)}, expected {tuple(shape)}")
+    if not t.is_cuda or (device is not None and t.get_device() != device):
+        raise ValueError(f"{name}: on {t.device}, expected {'a CUDA device' if device is None else f'cuda:{device}'}")
+    rows, cols = got
+    pitch, unit = t.stride()
+    if cols > 1 and unit != 1:
         raise ValueError(f"{name}: columns must be contiguous")
-    pitch = t.stride(0) if rows > 1 else max(cols, 1)
+    if rows == 1:
+        return max(cols, 1)
     if pitch < cols:
         raise ValueError(f"{name}: rows overlap (row stride {pitch})")
     return pitch
 
 
-def _flat(name: str, t: torch.Tensor, dtype, numel: int, device) -> None:
-    """Checks a contiguous tensor of at least `numel` elements."""
-    if t.dtype != dtype or t.device != device or not t.is_contiguous() or t.numel() < numel:
-        raise ValueError(f"{name}: needs {numel} contiguous {dtype} elements on {device}, got {t.numel()} of {t.dtype} "
-                         f"on {t.device}")
+def _flat(name: str, t: torch.Tensor, dtype, numel: int, device: int) -> None:
+    """Checks a contiguous tensor of at least `numel` elements on a CUDA device."""
+    if t.dtype != dtype or t.numel() < numel or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name}: needs {numel} contiguous {dtype} elements on cuda:{device}, got {t.numel()} of "
+                         f"{t.dtype} on {t.device}")
 
 
-def _empty(shape, dtype, device, stream) -> torch.Tensor:
+def _empty(shape, dtype, device: int, stream) -> torch.Tensor:
+    device = torch.device("cuda", device)
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
     if isinstance(stream, int):
@@ -309,14 +313,27 @@ def _empty(shape, dtype, device, stream) -> torch.Tensor:
         return torch.empty(shape, dtype=dtype, device=device)
 
 
-def _launch(name: str, fn, device, stream, *args) -> None:
-    """fn(*args, stream) with `device` current; `stream` None = that device's current stream."""
-    if isinstance(stream, torch.cuda.Stream) and stream.device != device:
-        raise ValueError(f"{name}: stream on {stream.device}, tensors on {device}")
-    if device.index != torch.cuda.current_device():
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _launch(name: str, fn, device: int, stream, *args) -> None:
+    """fn(*args, stream) with `device` current; `stream` None = that device's current stream, taken as a raw handle
+    (building the torch.cuda.Stream object costs as much as the launch)."""
+    if stream is None:
+        raw = _current_stream(device)
+    elif isinstance(stream, int):
+        raw = stream
+    else:
+        if stream.device.index != device:
+            raise ValueError(f"{name}: stream on {stream.device}, tensors on cuda:{device}")
+        raw = stream.cuda_stream
+    if device == _current_device():
+        code = fn(*args, raw)
+    else:
         with torch.cuda.device(device):
-            return _check(name, fn(*args, _stream(stream)))
-    _check(name, fn(*args, _stream(stream)))
+            code = fn(*args, raw)
+    if code != 0:
+        raise NvFp4Error(name, code)
 
 
 def mx_scale_buffer_bytes(outer: int, K: int) -> int:
@@ -326,24 +343,30 @@ def mx_scale_buffer_bytes(outer: int, K: int) -> int:
 
 def mx_swizzle_scales(logical: torch.Tensor, outer: int, K: int, stream=None) -> torch.Tensor:
     """Logical e8m0 scales [outer, K/32] uint8 (as a checkpoint holds them) -> tile layout."""
-    _flat("mx_swizzle_scales: logical", logical, torch.uint8, outer * (K // 32), logical.device)
-    out = _empty(mx_scale_buffer_bytes(outer, K), torch.uint8, logical.device, stream)
-    _launch("mx_swizzle_scales", _mx_sigs().nvfp4b_mx_swizzle_scales, logical.device, stream, _ptr(logical),
-            _ptr(out), outer, K)
+    if not logical.is_cuda:
+        raise ValueError(f"mx_swizzle_scales: logical: on {logical.device}, expected a CUDA device")
+    dev = logical.get_device()
+    _flat("mx_swizzle_scales: logical", logical, torch.uint8, outer * (K // 32), dev)
+    out = _empty(mx_scale_buffer_bytes(outer, K), torch.uint8, dev, stream)
+    _launch("mx_swizzle_scales", _mx_sigs().nvfp4b_mx_swizzle_scales, dev, stream, logical.data_ptr(),
+            out.data_ptr(), outer, K)
     return out
 
 
-def _mx_buffers(name, M, K, codes, scales, device, stream):
+_FLOATS = (torch.bfloat16, torch.float32)
+
+
+def _mx_buffers(name: str, M: int, K: int, codes, scales, device: int, stream):
     if K % 32:
         raise ValueError(f"{name}: width {K} is not a multiple of 32")
     if codes is None:
         codes = _empty((M, K // 2), torch.uint8, device, stream)
     else:
-        _flat(f"{name}: codes", codes, torch.uint8, M * (K // 2), device)
+        _flat(name + ": codes", codes, torch.uint8, M * (K // 2), device)
     if scales is None:
         scales = _empty(mx_scale_buffer_bytes(M, K), torch.uint8, device, stream)
     else:
-        _flat(f"{name}: scales", scales, torch.uint8, mx_scale_buffer_bytes(M, K), device)
+        _flat(name + ": scales", scales, torch.uint8, mx_scale_buffer_bytes(M, K), device)
     return codes, scales
 
 
@@ -352,10 +375,11 @@ def mx_quantize(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torc
     multiple of 16 bytes).  Returns (codes [M, K/2] uint8, tile-layout e8m0 scales uint8)."""
     ld = _rows("mx_quantize: x", x, (torch.bfloat16, torch.float32), (None, None))
     M, K = x.shape
-    codes, scales = _mx_buffers("mx_quantize", M, K, codes, scales, x.device, stream)
+    dev = x.get_device()
+    codes, scales = _mx_buffers("mx_quantize", M, K, codes, scales, dev, stream)
     L = _mx_sigs()
     fn = L.nvfp4b_mx_quantize_bf16 if x.dtype == torch.bfloat16 else L.nvfp4b_mx_quantize_f32
-    _launch("mx_quantize", fn, x.device, stream, _ptr(x), ld, M, K, _ptr(codes), _ptr(scales))
+    _launch("mx_quantize", fn, dev, stream, x.data_ptr(), ld, M, K, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -367,9 +391,10 @@ def mx_geglu_quantize(gate_up: torch.Tensor, codes: torch.Tensor | None = None, 
     M, I = gate_up.shape[0], gate_up.shape[1] // 2
     if gate_up.shape[1] % 2:
         raise ValueError("mx_geglu_quantize: odd width")
-    codes, scales = _mx_buffers("mx_geglu_quantize", M, I, codes, scales, gate_up.device, stream)
-    _launch("mx_geglu_quantize", _mx_sigs().nvfp4b_mx_geglu_quantize, gate_up.device, stream, _ptr(gate_up), ld, M, I,
-            _ptr(codes), _ptr(scales))
+    dev = gate_up.get_device()
+    codes, scales = _mx_buffers("mx_geglu_quantize", M, I, codes, scales, dev, stream)
+    _launch("mx_geglu_quantize", _mx_sigs().nvfp4b_mx_geglu_quantize, dev, stream, gate_up.data_ptr(), ld, M, I,
+            codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -377,13 +402,14 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype 
                   out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """The values of MXFP4 codes [M, K/2] and tile-layout scales as bf16 or fp32 [M, K] (exact in both)."""
     _rows("mx_dequantize: codes", codes, (torch.uint8,), (None, None))
-    M, K = codes.shape[0], 2 * codes.shape[1]
-    _mx_buffers("mx_dequantize", M, K, codes, scales, codes.device, stream)
+    M, half = codes.shape
+    K, dev = 2 * half, codes.get_device()
+    _mx_buffers("mx_dequantize", M, K, codes, scales, dev, stream)
     if out is None:
-        out = _empty((M, K), dtype, codes.device, stream)
-    ld = _rows("mx_dequantize: out", out, (torch.bfloat16, torch.float32), (M, K), codes.device)
-    _launch("mx_dequantize", _mx_sigs().nvfp4b_mx_dequantize, codes.device, stream, _ptr(codes), _ptr(scales), M, K,
-            _ptr(out), 1 if out.dtype == torch.float32 else 0, ld)
+        out = _empty((M, K), dtype, dev, stream)
+    ld = _rows("mx_dequantize: out", out, _FLOATS, (M, K), dev)
+    _launch("mx_dequantize", _mx_sigs().nvfp4b_mx_dequantize, dev, stream, codes.data_ptr(), scales.data_ptr(), M, K,
+            out.data_ptr(), 1 if out.dtype == torch.float32 else 0, ld)
     return out
 
 
@@ -394,8 +420,9 @@ def mx_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: 
     [M, N] bf16 or fp32 (rows may be strided), or fp32 [N, M] with OUT_F32_COLMAJOR, as in ``gemm``."""
     _rows("mx_gemm: a", a, (torch.uint8,), (None, None))
     M, half = a.shape
-    _rows("mx_gemm: b", b, (torch.uint8,), (None, half), a.device)
-    N, K, dev = b.shape[0], 2 * half, a.device
+    K, dev = 2 * half, a.get_device()
+    _rows("mx_gemm: b", b, (torch.uint8,), (None, half), dev)
+    N = b.shape[0]
     _mx_buffers("mx_gemm: a", M, K, a, a_scales, dev, stream)
     _mx_buffers("mx_gemm: b", N, K, b, b_scales, dev, stream)
     if out_kind not in (OUT_BF16_ROWMAJOR, OUT_F32_COLMAJOR, OUT_F32_ROWMAJOR):
@@ -405,8 +432,8 @@ def mx_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: 
     if out is None:
         out = _empty(shape, dtype, dev, stream)
     ldd = _rows("mx_gemm: out", out, (dtype,), shape, dev)
-    _launch("mx_gemm", _mx_sigs().nvfp4b_mx_gemm, dev, stream, _ptr(a), _ptr(a_scales), _ptr(b), _ptr(b_scales),
-            float(alpha), M, N, K, _ptr(out), out_kind, ldd)
+    _launch("mx_gemm", _mx_sigs().nvfp4b_mx_gemm, dev, stream, a.data_ptr(), a_scales.data_ptr(), b.data_ptr(),
+            b_scales.data_ptr(), float(alpha), M, N, K, out.data_ptr(), out_kind, ldd)
     return out
 
 
@@ -417,9 +444,6 @@ class BlockNorm(NamedTuple):
     amax: torch.Tensor | None
     codes: torch.Tensor | None
     scales: torch.Tensor | None
-
-
-_FLOATS = (torch.bfloat16, torch.float32)
 
 
 def block_norm(resid: torch.Tensor | None = None, norm_weight: torch.Tensor | None = None, eps: float = 1e-6,
@@ -442,8 +466,10 @@ def block_norm(resid: torch.Tensor | None = None, norm_weight: torch.Tensor | No
     if x.dim() != 2:
         raise ValueError(f"block_norm: shape {tuple(x.shape)}, expected [T, H]")
     T, H = x.shape
-    dev, a = x.device, _BlockNormArgs()
-    a.T, a.H, a.scale, a.eps = T, H, scale, eps
+    if not x.is_cuda:
+        raise ValueError(f"block_norm: on {x.device}, expected a CUDA device")
+    dev, a = x.get_device(), _BlockNormArgs(T, H)
+    a.scale, a.eps = scale, eps
     mx = mx or codes is not None or scales is not None
     if resid is not None:
         a.ld_resid = _rows("block_norm: resid", resid, _FLOATS, (T, H), dev)
@@ -460,9 +486,9 @@ def block_norm(resid: torch.Tensor | None = None, norm_weight: torch.Tensor | No
         a.post_weight = post_weight.data_ptr()
     a.post_norm = post_weight is not None if post_norm is None else bool(post_norm)
     if gate is not None:
-        if gate.dtype not in _FLOATS or gate.device != dev or tuple(gate.shape) not in ((H,), (T, 1), (T, H)):
+        if gate.dtype not in _FLOATS or gate.get_device() != dev or tuple(gate.shape) not in ((H,), (T, 1), (T, H)):
             raise ValueError(f"block_norm: gate {tuple(gate.shape)} {gate.dtype} on {gate.device}, expected bf16 or fp32 "
-                             f"[{H}], [{T}, 1] or [{T}, {H}] on {dev}")
+                             f"[{H}], [{T}, 1] or [{T}, {H}] on cuda:{dev}")
         cols = gate.shape[-1] > 1 or H == 1
         if cols and gate.stride(-1) != 1:
             raise ValueError("block_norm: gate: columns must be contiguous")

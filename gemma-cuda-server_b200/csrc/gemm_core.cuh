@@ -235,6 +235,39 @@ __device__ __forceinline__ void issue_scale_copies(int part, int tiles, uint32_t
     }
 }
 
+// The MMAs of one K-tile: `nks` steps of 32 operand bytes, descriptors advanced by addition (32 bytes = 2 in the address
+// field; the shared-memory window keeps the sum inside it).  Whole K-tiles take the unrolled form: the one issuing
+// thread's own instructions, not the tensor pipe, were what a K-tile waited for.
+template <class C, bool PAIR>
+__device__ __forceinline__ void issue_mma(uint32_t d_tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa,
+                                          uint32_t sfb, int j, uint32_t acc) {
+    using namespace sm100;
+    if constexpr (C::KIND == Kind::MXF4) {
+        const uint32_t id = idesc | ((j & 1) ? kMxScaleId2 : 0u), ca = sfa + 4 * (j >> 1), cb = sfb + (C::BN / 32) * (j >> 1);
+        if constexpr (PAIR) mma_mxf4_pair(d_tmem, ad + 2 * j, bd + 2 * j, id, ca, cb, acc);
+        else mma_mxf4(d_tmem, ad + 2 * j, bd + 2 * j, id, ca, cb, acc);
+    } else if constexpr (C::KIND == Kind::NVF4) {
+        const uint32_t ca = sfa + 4 * j, cb = sfb + (C::BN / 32) * j;
+        if constexpr (PAIR) mma_nvf4_pair(d_tmem, ad + 2 * j, bd + 2 * j, idesc, ca, cb, acc);
+        else mma_nvf4(d_tmem, ad + 2 * j, bd + 2 * j, idesc, ca, cb, acc);
+    } else {
+        mma_bf16(d_tmem, ad + 2 * j, bd + 2 * j, idesc, acc);
+    }
+}
+
+template <class C, bool PAIR>
+__device__ __forceinline__ void issue_k_tile(uint32_t d_tmem, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t sfa,
+                                             uint32_t sfb, int nks, uint32_t acc0) {
+    if (nks == 4) {
+        issue_mma<C, PAIR>(d_tmem, ad, bd, idesc, sfa, sfb, 0, acc0);
+#pragma unroll
+        for (int j = 1; j < 4; ++j) issue_mma<C, PAIR>(d_tmem, ad, bd, idesc, sfa, sfb, j, 1u);
+    } else {
+#pragma unroll 1
+        for (int j = 0; j < nks; ++j) issue_mma<C, PAIR>(d_tmem, ad, bd, idesc, sfa, sfb, j, (acc0 | j) != 0 ? 1u : 0u);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------------------------
 // The kernel
 // ---------------------------------------------------------------------------------------------------------------
@@ -312,6 +345,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             bool ok = true;
             const uint32_t sfa_col = tmem + (uint32_t)C::SF_COL0;
             const uint32_t sfb_col = sfa_col + C::SF_COLS_A;
+            const uint64_t a_desc = desc_kmajor_sw128(smem_u32(sA)), b_desc = desc_kmajor_sw128(smem_u32(sB));
             for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
                 const TileInfo ti = sched.tile(t);
                 const uint32_t idesc = C::KIND == Kind::NVF4   ? idesc_nvf4(C::BM, ti.n_mma)
@@ -323,30 +357,14 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 for (int kt = ti.kt0; kt < ti.kt1; ++kt) {
                     if (!mbar_wait(&full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
                     tc_fence_after();
-                    const int nks = k_steps<C>(cp, kt);
-                    const uint32_t a_base = smem_u32(sA + stage * C::A_BYTES);
-                    const uint32_t b_base = smem_u32(sB + stage * C::B_BYTES);
-                    const uint32_t acc0 = kt != ti.kt0 ? 1u : 0u;
+                    const uint64_t ad = a_desc + stage * (C::A_BYTES >> 4), bd = b_desc + stage * (C::B_BYTES >> 4);
+                    const uint32_t so = (uint32_t)(stage * (C::SF_COLS_A + C::SF_COLS_B));
                     if constexpr (C::SCALED) {
                         if (!mbar_wait(&sf_full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
                         tc_fence_after();
-                        const uint32_t so = (uint32_t)(stage * (C::SF_COLS_A + C::SF_COLS_B));
-                        for (int j = 0; j < nks; ++j) {
-                            const uint64_t ad = desc_kmajor_sw128(a_base + 32 * j);
-                            const uint64_t bd = desc_kmajor_sw128(b_base + 32 * j);
-                            const uint32_t acc = (acc0 | j) != 0 ? 1u : 0u;
-                            if constexpr (C::KIND == Kind::MXF4)
-                                mma_mxf4(d_tmem, ad, bd, idesc | ((j & 1) ? kMxScaleId2 : 0u),
-                                         sfa_col + so + 4 * (j >> 1), sfb_col + so + (C::BN / 32) * (j >> 1), acc);
-                            else
-                                mma_nvf4(d_tmem, ad, bd, idesc, sfa_col + so + 4 * j, sfb_col + so + (C::BN / 32) * j,
-                                         acc);
-                        }
-                    } else {
-                        for (int j = 0; j < nks; ++j)
-                            mma_bf16(d_tmem, desc_kmajor_sw128(a_base + 32 * j), desc_kmajor_sw128(b_base + 32 * j),
-                                     idesc, (acc0 | j) != 0 ? 1u : 0u);
                     }
+                    issue_k_tile<C, false>(d_tmem, ad, bd, idesc, sfa_col + so, sfb_col + so, k_steps<C>(cp, kt),
+                                           kt != ti.kt0 ? 1u : 0u);
                     tc_commit(&empty[stage]);
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
                 }
@@ -572,7 +590,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             const uint32_t sfb_col = sfa_col + C::SF_COLS_A;
             const uint32_t idesc =
                 C::KIND == Kind::MXF4 ? idesc_mxf4(C::PAIR_M, C::BN) : idesc_nvf4(C::PAIR_M, C::BN);
-            const uint32_t tfull_own = smem_u32(tfull), tfull_peer = mapa_shared(smem_u32(tfull), 1);
+            const uint64_t a_desc = desc_kmajor_sw128(smem_u32(sA)), b_desc = desc_kmajor_sw128(smem_u32(sB));
             for (int t = cluster; t < num_tiles && ok; t += clusters) {
                 const TileInfo ti = sched.tile(t);
                 if (!mbar_wait_cluster(tempty, aphase ^ 1u, sflag, kErrTimeoutMma)) break;
@@ -580,31 +598,16 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 for (int kt = ti.kt0; kt < ti.kt1; ++kt) {
                     if (!mbar_wait(&full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
                     tc_fence_after();
-                    const int nks = k_steps<C>(cp, kt);
-                    const uint32_t a_base = smem_u32(sA + stage * C::A_BYTES);
-                    const uint32_t b_base = smem_u32(sB + stage * C::B_BYTES);
-                    const uint32_t acc0 = kt != ti.kt0 ? 1u : 0u;
                     if (!mbar_wait(&sf_full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t so = (uint32_t)(stage * (C::SF_COLS_A + C::SF_COLS_B));
-                    for (int j = 0; j < nks; ++j) {
-                        const uint64_t ad = desc_kmajor_sw128(a_base + 32 * j);
-                        const uint64_t bd = desc_kmajor_sw128(b_base + 32 * j);
-                        const uint32_t acc = (acc0 | j) != 0 ? 1u : 0u;
-                        if constexpr (C::KIND == Kind::MXF4)
-                            mma_mxf4_pair(tmem, ad, bd, idesc | ((j & 1) ? kMxScaleId2 : 0u),
-                                          sfa_col + so + 4 * (j >> 1), sfb_col + so + 8 * (j >> 1), acc);
-                        else
-                            mma_nvf4_pair(tmem, ad, bd, idesc, sfa_col + so + 4 * j, sfb_col + so + 8 * j, acc);
-                    }
-                    const uint32_t eb = smem_u32(&empty[stage]);
-                    tc_commit_pair(eb);
-                    tc_commit_pair(mapa_shared(eb, 1));
+                    issue_k_tile<C, true>(tmem, a_desc + stage * (C::A_BYTES >> 4), b_desc + stage * (C::B_BYTES >> 4),
+                                          idesc, sfa_col + so, sfb_col + so, k_steps<C>(cp, kt), kt != ti.kt0 ? 1u : 0u);
+                    tc_commit_both(&empty[stage]);
                     if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
                 }
                 if (!ok) break;
-                tc_commit_pair(tfull_own);
-                tc_commit_pair(tfull_peer);
+                tc_commit_both(tfull);
                 aphase ^= 1u;
             }
         }

@@ -361,6 +361,16 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar_cluster) {
                  : "memory");
 }
 
+// Arrive once on `bar` in both CTAs of the pair (the same shared-memory offset) when the pair operations issued so far
+// complete.  (A completion signal only: no data is multicast.)
+__device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
 // ---- descriptors ---------------------------------------------------------------------------------------------
 
 // K-major operand tile written by TMA with 128-byte swizzle: rows of 128 bytes, 8-row atoms 1024 bytes apart.
