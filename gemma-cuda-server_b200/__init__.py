@@ -356,6 +356,19 @@ def mx_swizzle_scales(logical: torch.Tensor, outer: int, K: int, stream=None) ->
 _FLOATS = (torch.bfloat16, torch.float32)
 
 
+def _mx_operand(name: str, codes: torch.Tensor, scales: torch.Tensor, device: int | None = None):
+    """Checks MXFP4 codes [rows, K/2] with their tile-layout scales; returns rows, K and the device index."""
+    if codes.dim() != 2:
+        raise ValueError(f"{name}: shape {tuple(codes.shape)}, expected [rows, K/2]")
+    M, half = codes.shape
+    if device is None:
+        device = codes.get_device()
+        if device < 0:
+            raise ValueError(f"{name}: on {codes.device}, expected a CUDA device")
+    _mx_buffers(name, M, 2 * half, codes, scales, device, None)
+    return M, 2 * half, device
+
+
 def _mx_buffers(name: str, M: int, K: int, codes, scales, device: int, stream):
     if K % 32:
         raise ValueError(f"{name}: width {K} is not a multiple of 32")
@@ -401,10 +414,7 @@ def mx_geglu_quantize(gate_up: torch.Tensor, codes: torch.Tensor | None = None, 
 def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
                   out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """The values of MXFP4 codes [M, K/2] and tile-layout scales as bf16 or fp32 [M, K] (exact in both)."""
-    _rows("mx_dequantize: codes", codes, (torch.uint8,), (None, None))
-    M, half = codes.shape
-    K, dev = 2 * half, codes.get_device()
-    _mx_buffers("mx_dequantize", M, K, codes, scales, dev, stream)
+    M, K, dev = _mx_operand("mx_dequantize", codes, scales)
     if out is None:
         out = _empty((M, K), dtype, dev, stream)
     ld = _rows("mx_dequantize: out", out, _FLOATS, (M, K), dev)
@@ -418,13 +428,10 @@ def mx_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: 
             stream=None) -> torch.Tensor:
     """D = alpha * A @ B^T on the MXFP4 tensor cores.  A: codes [M, K/2]; B: codes [N, K/2]; tile-layout scales.  D is
     [M, N] bf16 or fp32 (rows may be strided), or fp32 [N, M] with OUT_F32_COLMAJOR, as in ``gemm``."""
-    _rows("mx_gemm: a", a, (torch.uint8,), (None, None))
-    M, half = a.shape
-    K, dev = 2 * half, a.get_device()
-    _rows("mx_gemm: b", b, (torch.uint8,), (None, half), dev)
-    N = b.shape[0]
-    _mx_buffers("mx_gemm: a", M, K, a, a_scales, dev, stream)
-    _mx_buffers("mx_gemm: b", N, K, b, b_scales, dev, stream)
+    M, K, dev = _mx_operand("mx_gemm: a", a, a_scales)
+    N, kb, _ = _mx_operand("mx_gemm: b", b, b_scales, dev)
+    if kb != K:
+        raise ValueError(f"mx_gemm: b: shape {tuple(b.shape)}, expected [N, {K // 2}]")
     if out_kind not in (OUT_BF16_ROWMAJOR, OUT_F32_COLMAJOR, OUT_F32_ROWMAJOR):
         raise ValueError(f"mx_gemm: unknown out_kind {out_kind}")
     shape = (N, M) if out_kind == OUT_F32_COLMAJOR else (M, N)

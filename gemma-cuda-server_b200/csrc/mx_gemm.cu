@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "dense_epi.cuh"
 #include "gemm_core.cuh"
@@ -22,7 +24,6 @@ struct MxGemm {
     long long ldd;
 };
 
-using MxTile = KCfg<256, 4, 1, 8, Kind::MXF4>;
 using MxPair = PairCfg<5, 8, 8 * kStoreTileBytes, Kind::MXF4>;   // + bf16 store staging tiles
 
 template <class Epi>
@@ -48,27 +49,386 @@ int mx_core_params(const MxGemm& g, CoreParams& cp) {
     return NVFP4B_OK;
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows: the weights as the M = 128 operand
+// ---------------------------------------------------------------------------------------------------------------
+// D^T = B A^T: 128 rows of B (the weights) against NT = 16, 32, 64 or 128 rows of A.  What a call of few rows does is
+// stream the weights, so the tile is narrow in A's rows (the tensor pipe and the epilogue do no work for padding) and K
+// is split over the S CTAs of a cluster while there are fewer tiles than SMs; the partial sums meet in distributed shared
+// memory, each CTA adding up every S-th row in rank order (the same bits every time, no workspace).  One CTA per SM with
+// about 200 KB of stages; persistent over tiles when S = 1, with two accumulators.
+//   warp 0      producer: TMA loads of the weights (128 x 128 bytes) and of A (NT x 128 bytes), bulk loads of the scales
+//   warp 1      TMEM owner and MMA issuer
+//   warps 2-5   epilogue, TMEM lane quadrant warp % 4: a thread holds one column n of D for all rows of the tile; 16 rows
+//               at a time are turned around in shared memory so that a lane stores 16 bytes
+//   warp 6      scale copies (issued by the MMA thread they made a K-tile take 1330 cycles)
+template <int NT_>
+struct SkinnyCfg {
+    static constexpr int NT = NT_, A_BYTES = NT * 128, W_BYTES = 128 * 128, SF_BYTES = 2 * 512;
+    static constexpr int STAGE_BYTES = W_BYTES + A_BYTES + 2 * SF_BYTES;
+    static constexpr int STAGES = 208 * 1024 / STAGE_BYTES;
+    static constexpr int BAR_BYTES = 384;
+    static constexpr int TURN = 33, TURN_BYTES = 4 * 16 * TURN * 4;   // per epilogue warp: 16 rows x 32 columns, padded
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + BAR_BYTES + TURN_BYTES + 1024;
+    static constexpr int SF_COL0 = 2 * NT, SF_COLS = 16;          // per stage: 8 columns for the weights, 8 for A
+    static constexpr int PART = 132;                              // row pitch of the partial sums, floats
+    static constexpr int THREADS = 224;
+    static_assert(SF_COL0 + STAGES * SF_COLS <= 512, "TMEM budget");
+    static_assert((3 * STAGES + 4) * 8 + 16 <= BAR_BYTES, "barriers");
+    static_assert(NT * PART * 4 <= STAGES * STAGE_BYTES, "partial sums");
+    static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+};
+
+// What issue_k_tile takes from its configuration.
+template <int NT>
+struct MmaOf {
+    static constexpr Kind KIND = Kind::MXF4;
+    static constexpr int BN = 128;                                // columns of one scale tile's copy: 4
+};
+
+struct SkinnyParams {
+    const uint8_t *sfa, *sfw;
+    void* d;
+    long long ldd;
+    float alpha;
+    int M, N, n_tiles, m_tiles, tile_cols, k_steps, k_tiles;
+    int wide;                // d and its pitch allow 16-byte stores
+    int* err;
+};
+
 template <int OUT>
-int mx_run_tile(const MxGemm& g, cudaStream_t stream) {
-    using C = MxTile;
-    CUtensorMap ma, mb;
-    int st = make_kmajor_map(&ma, g.a, g.M, g.K / 2, C::BM);
+__device__ __forceinline__ void skinny_store(const SkinnyParams& p, int m, int n, float v) {
+    v *= p.alpha;
+    if constexpr (OUT == NVFP4B_OUT_BF16_ROWMAJOR) static_cast<__nv_bfloat16*>(p.d)[m * p.ldd + n] = __float2bfloat16_rn(v);
+    else if constexpr (OUT == NVFP4B_OUT_F32_ROWMAJOR) static_cast<float*>(p.d)[m * p.ldd + n] = v;
+    else static_cast<float*>(p.d)[n * p.ldd + m] = v;
+}
+
+// One warp stores rows m0.. (16 of them, `rows` exist) x columns n0.. (32) of D; lane = column in r, turned around in `t`.
+template <int OUT>
+__device__ __forceinline__ void skinny_store16(const SkinnyParams& p, int m0, int rows, int n0, const uint32_t (&r)[16],
+                                               float* t) {
+    constexpr int P = SkinnyCfg<16>::TURN;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i * P + lane] = p.alpha * __uint_as_float(r[i]);
+    __syncwarp();
+    if constexpr (OUT == NVFP4B_OUT_F32_COLMAJOR) {               // a lane stores four rows of one column
+        const bool whole = p.wide && rows >= 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = i * 8 + (lane >> 2), m = 4 * (lane & 3);
+            float* d = static_cast<float*>(p.d) + (long long)(n0 + n) * p.ldd + m0 + m;
+            if (n0 + n >= p.N) continue;
+            if (whole) *reinterpret_cast<float4*>(d) = make_float4(t[m * P + n], t[(m + 1) * P + n], t[(m + 2) * P + n], t[(m + 3) * P + n]);
+            else
+                for (int e = 0; e < 4; ++e)
+                    if (m + e < rows) d[e] = t[(m + e) * P + n];
+        }
+    } else {
+        if (!p.wide || n0 + 32 > p.N) {                           // a lane stores its own column, row by row
+            if (n0 + lane < p.N)
+                for (int i = 0; i < min(rows, 16); ++i) {
+                    const long long at = (long long)(m0 + i) * p.ldd + n0 + lane;
+                    if constexpr (OUT == NVFP4B_OUT_BF16_ROWMAJOR) static_cast<__nv_bfloat16*>(p.d)[at] = __float2bfloat16_rn(t[i * P + lane]);
+                    else static_cast<float*>(p.d)[at] = t[i * P + lane];
+                }
+            __syncwarp();
+            return;
+        }
+        constexpr int kPer = OUT == NVFP4B_OUT_BF16_ROWMAJOR ? 8 : 4, kLanes = 32 / kPer;   // columns per lane, lanes per row
+#pragma unroll
+        for (int i = 0; i < 16 * kLanes / 32; ++i) {
+            const int m = i * (32 / kLanes) + lane / kLanes, n = kPer * (lane % kLanes);
+            const float* v = t + m * P + n;
+            if (m >= rows) continue;
+            if constexpr (OUT == NVFP4B_OUT_BF16_ROWMAJOR) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                    w[e] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.d) + (long long)(m0 + m) * p.ldd + n0 + n) =
+                    make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+                *reinterpret_cast<float4*>(static_cast<float*>(p.d) + (long long)(m0 + m) * p.ldd + n0 + n) =
+                    make_float4(v[0], v[1], v[2], v[3]);
+            }
+        }
+    }
+    __syncwarp();
+}
+
+// Sum, in rank order, of the four fp32 at one shared-memory address of the S <= 8 CTAs of the cluster; every load is issued
+// before the first addition waits for one.
+__device__ __forceinline__ float4 cluster_sum(uint32_t addr, int S) {
+    float4 x[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+        x[q] = q < S ? sm100::ld_cluster_f32x4(sm100::mapa_shared(addr, (uint32_t)q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int q = 1; q < 8; ++q) { x[0].x += x[q].x; x[0].y += x[q].y; x[0].z += x[q].z; x[0].w += x[q].w; }
+    return x[0];
+}
+
+template <int NT, int OUT>
+__global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 1)
+    mx_skinny_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_w,
+                     const __grid_constant__ SkinnyParams p) {
+    using namespace sm100;
+    using C = SkinnyCfg<NT>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sW = smem;
+    uint8_t* sA = sW + C::STAGES * C::W_BYTES;
+    uint8_t* sSF = sA + C::STAGES * C::A_BYTES;                   // per stage: weight scales, then A's
+    uint64_t* full = reinterpret_cast<uint64_t*>(sSF + C::STAGES * 2 * C::SF_BYTES);
+    uint64_t* empty = full + C::STAGES;
+    uint64_t* tfull = empty + C::STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint64_t* sf_full = tempty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sf_full + C::STAGES);
+    volatile int* sflag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* turn = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(full) + C::BAR_BYTES);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); mbar_init(&sf_full[s], 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 128); }
+        *sflag = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tma_a);
+        prefetch_tmap(&tma_w);
+    }
+    if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int tiles = p.n_tiles * p.m_tiles;
+    const int t0 = (int)blockIdx.x / S, step = (int)gridDim.x / S;
+    const int kt0 = p.k_tiles * rank / S, kt1 = p.k_tiles * (rank + 1) / S;   // none empty: S <= k_tiles
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = t0; t < tiles && ok; t += step) {
+                const int nb = t / p.m_tiles, mb = t - nb * p.m_tiles;
+                for (int kt = kt0; kt < kt1; ++kt) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1u, sflag, kErrTimeoutProducer)) { ok = false; break; }
+                    const uint32_t sf = 512u * (uint32_t)min(2, p.tile_cols - 2 * kt);
+                    uint8_t* f = sSF + stage * 2 * C::SF_BYTES;
+                    mbar_arrive_expect_tx(&full[stage], C::W_BYTES + C::A_BYTES + 2 * sf);
+                    tma_load_2d(sW + stage * C::W_BYTES, &tma_w, &full[stage], kt * 128, nb * 128);
+                    bulk_load(f, p.sfw + ((long long)nb * p.tile_cols + 2 * kt) * 512, sf, &full[stage]);
+                    tma_load_2d(sA + stage * C::A_BYTES, &tma_a, &full[stage], kt * 128, mb * NT);
+                    bulk_load(f + C::SF_BYTES, p.sfa + ((long long)mb * p.tile_cols + 2 * kt) * 512, sf, &full[stage]);
+                    if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int stage = 0, buf = 0;
+            uint32_t phase = 0, aphase = 0;
+            bool ok = true;
+            constexpr uint32_t idesc = idesc_mxf4(128, NT);
+            const uint64_t w_desc = desc_kmajor_sw128(smem_u32(sW)), a_desc = desc_kmajor_sw128(smem_u32(sA));
+            for (int t = t0; t < tiles && ok; t += step) {
+                if (!mbar_wait(&tempty[buf], aphase ^ 1u, sflag, kErrTimeoutMma)) break;
+                tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(buf * NT);
+                for (int kt = kt0; kt < kt1; ++kt) {
+                    if (!mbar_wait(&full[stage], phase, sflag, kErrTimeoutMma) ||
+                        !mbar_wait(&sf_full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t fw = tmem + (uint32_t)(C::SF_COL0 + stage * C::SF_COLS);
+                    issue_k_tile<MmaOf<NT>, false>(d, w_desc + stage * (C::W_BYTES >> 4), a_desc + stage * (C::A_BYTES >> 4),
+                                                   idesc, fw, fw + 8, min(4, p.k_steps - 4 * kt), kt != kt0 ? 1u : 0u);
+                    tc_commit(&empty[stage]);
+                    if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                }
+                if (!ok) break;
+                tc_commit(&tfull[buf]);
+                buf ^= 1;
+                if (buf == 0) aphase ^= 1u;
+            }
+        }
+    } else if (warp == 6) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            const uint64_t f_desc = desc_sf_32x16(smem_u32(sSF));
+            for (int t = t0; t < tiles && ok; t += step) {
+                for (int kt = kt0; kt < kt1; ++kt) {
+                    if (!mbar_wait(&full[stage], phase, sflag, kErrTimeoutMma)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t fd = f_desc + stage * (2 * C::SF_BYTES >> 4);
+                    const uint32_t fw = tmem + (uint32_t)(C::SF_COL0 + stage * C::SF_COLS);
+                    const int sf = min(2, p.tile_cols - 2 * kt);
+                    for (int j = 0; j < sf; ++j) {
+                        tmem_cp_32x128b_x4(fw + 4 * j, fd + j * (512 >> 4));
+                        tmem_cp_32x128b_x4(fw + 8 + 4 * j, fd + ((C::SF_BYTES + j * 512) >> 4));
+                    }
+                    tc_commit(&sf_full[stage]);
+                    if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+    } else {
+        const int quad = warp & 3, col = quad * 32 + lane;        // column of D within the tile
+        int buf = 0;
+        uint32_t aphase = 0;
+        for (int t = t0; t < tiles; t += step) {
+            const int nb = t / p.m_tiles, mb = t - nb * p.m_tiles;
+            const int m0 = mb * NT, rows = min(NT, p.M - m0);
+            if (!mbar_wait(&tfull[buf], aphase, sflag, kErrTimeoutEpilogue)) break;
+            tc_fence_after();
+            const uint32_t addr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * NT);
+#pragma unroll 1
+            for (int c0 = 0; c0 < rows; c0 += 16) {
+                uint32_t r[16];
+                tmem_ld_32x32b_x16(addr + c0, r);
+                tmem_wait_ld();
+                if (S == 1) {
+                    skinny_store16<OUT>(p, m0 + c0, rows - c0, nb * 128 + quad * 32, r, turn + quad * 16 * C::TURN);
+                } else {                                          // the stages are free: every load and MMA is done
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) reinterpret_cast<uint32_t*>(smem)[(c0 + i) * C::PART + col] = r[i];
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(&tempty[buf]);
+            buf ^= 1;
+            if (buf == 0) aphase ^= 1u;
+        }
+    }
+    if (S > 1) {                                                  // one tile per cluster
+        cluster_sync();
+        const int nb = t0 / p.m_tiles, mb = t0 - nb * p.m_tiles;
+        const int rows = min(NT, p.M - mb * NT), e = (warp - 2) & 3;
+        const uint32_t base = smem_u32(smem);
+        if (warp >= 2 && warp < 6) {
+            // Row-major D: a warp takes a row of the tile, four columns per lane.  Column-major: four columns of the tile,
+            // a row per lane.  Either way the lanes' pieces lie together in D, and the padded pitch keeps the 16-byte
+            // reads of a quarter-warp on distinct banks.
+            constexpr bool COL = OUT == NVFP4B_OUT_F32_COLMAJOR;
+            const int items = COL ? 32 * ((rows + 31) / 32) : rows;
+            for (int i = rank * 4 + e; i < items; i += 4 * S) {
+                const int c = COL ? (i >> 5) * 32 + lane : i, n = 4 * (COL ? i & 31 : lane);
+                if (COL && c >= rows) continue;
+                const float4 v = cluster_sum(base + 4u * (uint32_t)(c * C::PART + n), S);
+                const int gm = mb * NT + c, gn = nb * 128 + n;
+                const float x[4] = {v.x, v.y, v.z, v.w};
+                if (!COL && p.wide && gn + 4 <= p.N) {
+                    if constexpr (OUT == NVFP4B_OUT_BF16_ROWMAJOR) {
+                        const __nv_bfloat162 h0 = __floats2bfloat162_rn(p.alpha * x[0], p.alpha * x[1]);
+                        const __nv_bfloat162 h1 = __floats2bfloat162_rn(p.alpha * x[2], p.alpha * x[3]);
+                        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.d) + gm * p.ldd + gn) =
+                            make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+                    } else {
+                        *reinterpret_cast<float4*>(static_cast<float*>(p.d) + gm * p.ldd + gn) =
+                            make_float4(p.alpha * x[0], p.alpha * x[1], p.alpha * x[2], p.alpha * x[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (gn + k < p.N) skinny_store<OUT>(p, gm, gn + k, x[k]);
+                }
+            }
+        }
+        cluster_sync();                                           // no CTA leaves while a peer reads its sums
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+    if (threadIdx.x == 0 && *sflag != 0) atomicCAS(p.err, 0, *sflag);
+}
+
+// The CTAs that K is split over.  A split saves a CTA k_tiles (1 - 1/S) K-tiles of about 0.27 us and costs the meeting of
+// the partial sums, which grows with the tile's rows and is twice as dear column-major (N = 2816: 16 rows, K = 2816, S = 6
+// 5.2 against 7.3 us unsplit; 128 rows 8.1 and 9.3; K = 704, S = 3 4.9 and 4.6, 8.1 and 6.7), so it is taken from 3 +
+// NT / 32 saved K-tiles on, and only as far as all clusters are resident at once (24 clusters of 6 are not: 14.4 us
+// against 8.4 with 4).
+template <int NT>
+int skinny_split(int tiles, int k_tiles, bool col, const std::atomic<int> (&resident)[9]) {
+    const int need = (3 + NT / 32) * (col ? 2 : 1);
+    for (int S = k_tiles < 8 ? k_tiles : 8; S > 1; --S)
+        if (tiles <= resident[S].load(std::memory_order_relaxed) && k_tiles * (S - 1) >= need * S) return S;
+    return 1;
+}
+
+template <int NT, int OUT>
+int mx_run_skinny(const MxGemm& g, cudaStream_t stream) {
+    using C = SkinnyCfg<NT>;
+    const auto kernel = mx_skinny_kernel<NT, OUT>;
+    static std::atomic<bool> ready[64];                // per device: shared-memory limit raised, resident[] filled (host
+    static std::atomic<int> resident[64][9];           // threads may race to, with the same values): clusters of S at once
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return NVFP4B_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(C::THREADS, 1, 1);
+    cfg.dynamicSmemBytes = C::SMEM_BYTES;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+        if (e != cudaSuccess) return record_cuda_error(e);
+        for (int S = 2; S <= 8; ++S) {
+            attr[0].val.clusterDim.x = (unsigned)S;
+            cfg.gridDim = dim3((unsigned)(S * 148), 1, 1);
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+                cudaGetLastError();                    // this size is not taken
+                n = 0;
+            }
+            resident[dev][S].store(n, std::memory_order_relaxed);
+        }
+        ready[dev].store(true, std::memory_order_release);
+    }
+    CUtensorMap ma, mw;
+    int st = make_kmajor_map(&ma, g.a, g.M, g.K / 2, NT);
     if (st) return st;
-    st = make_kmajor_map(&mb, g.b, g.N, g.K / 2, C::BN);
+    st = make_kmajor_map(&mw, g.b, g.N, g.K / 2, 128);
     if (st) return st;
-    CoreParams cp;
-    st = mx_core_params(g, cp);
-    if (st) return st;
-    DenseSched<C::BN> s;
-    s.m_tiles = (g.M + C::BM - 1) / C::BM;
-    s.n_tiles = (g.N + C::BN - 1) / C::BN;
-    s.group_m = 16;
-    s.N = g.N;
-    s.b_row_tiles = (g.N + 127) / 128;
-    s.k_tiles = cp.k_tiles;
-    const int tiles = s.m_tiles * s.n_tiles;
-    const int grid = tiles < sm_count() ? tiles : sm_count();
-    return launch_core<C>(ma, mb, cp, s, mx_epilogue<DenseEpi<OUT>>(g), grid, stream);
+    SkinnyParams p;
+    p.sfa = g.a_sf;
+    p.sfw = g.b_sf;
+    p.d = g.d;
+    p.ldd = g.ldd;
+    p.alpha = g.alpha;
+    p.M = g.M;
+    p.N = g.N;
+    p.n_tiles = (g.N + 127) / 128;
+    p.m_tiles = (g.M + NT - 1) / NT;
+    p.tile_cols = (g.K + 127) / 128;
+    p.k_steps = (g.K + 63) / 64;
+    p.k_tiles = (g.K + 255) / 256;
+    p.wide = g.ldd % (OUT == NVFP4B_OUT_BF16_ROWMAJOR ? 8 : 4) == 0;     // d is 16-byte aligned
+    p.err = device_error_ptr();
+    if (!p.err) return NVFP4B_ERR_CUDA;
+    const long long tiles = (long long)p.n_tiles * p.m_tiles;
+    if (tiles > (1ll << 30)) return NVFP4B_ERR_SHAPE;
+    const int sms = sm_count();
+    const int S = tiles >= sms ? 1 : skinny_split<NT>((int)tiles, p.k_tiles, OUT == NVFP4B_OUT_F32_COLMAJOR, resident[dev]);
+    attr[0].val.clusterDim.x = (unsigned)S;
+    cfg.gridDim = dim3((unsigned)(S > 1 ? tiles * S : tiles < sms ? tiles : sms), 1, 1);
+    cfg.stream = stream;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, ma, mw, p);
+    return err == cudaSuccess ? NVFP4B_OK : record_cuda_error(err);
 }
 
 template <int OUT>
@@ -94,9 +454,16 @@ int mx_run_pair(const MxGemm& g, cudaStream_t stream) {
     return launch_pair<C>(ma, mb, msa, msb, cp, s, mx_epilogue<DenseEpi<OUT, true>>(g), s.m_tiles * s.n_tiles, stream);
 }
 
+// The narrow tiles up to 128 rows, and above as long as they make one round (K = 2816: 512 x 4224 9.7 us against 11.1 in
+// CTA-pair tiles, 256 x 8448 10.0 and 11.3; 512 x 8448, two rounds, 14.9 and 12.3).
 template <int OUT>
 int mx_run(const MxGemm& g, cudaStream_t stream) {
-    return g.M > 128 ? mx_run_pair<OUT>(g, stream) : mx_run_tile<OUT>(g, stream);
+    if (g.M <= 16) return mx_run_skinny<16, OUT>(g, stream);
+    if (g.M <= 32) return mx_run_skinny<32, OUT>(g, stream);
+    if (g.M <= 64) return mx_run_skinny<64, OUT>(g, stream);
+    const long long tiles = ((long long)g.N + 127) / 128 * ((g.M + 127) / 128);
+    if (g.M <= 128 || tiles <= sm_count()) return mx_run_skinny<128, OUT>(g, stream);
+    return mx_run_pair<OUT>(g, stream);
 }
 
 }  // namespace
