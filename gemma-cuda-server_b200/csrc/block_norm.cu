@@ -7,7 +7,7 @@
 // bulk copies into a ring of two shared-memory stages, so the next row is on its way while this one goes through its
 // two or three block-wide barriers (a first version with a CTA per row and loads into registers spent its time
 // waiting: 148 us for 8192 x 2816 bf16 with a gate to MXFP4).  NCH chunks per thread: 4 at many rows (small CTAs,
-// several per SM), 1 at few (the shortest path through one row).
+// several per SM), 1 at few (the shortest path through a row).
 //
 // The codes stored are those of the float64 z.  With u = 2^-24 a sum of squares is off by at most 17 u of itself (4
 // fused steps and a join per chunk, 3 chunk joins, 5 + 4 tree levels), 1 / rms by 10 u, r by 15 u a with a = |scale|
@@ -34,7 +34,6 @@ __host__ __device__ constexpr int src_size(Src s) { return s == kF32 ? 4 : s == 
 constexpr int kNormMaxThreads = 512;
 constexpr int kNormMaxSmem = 220 * 1024;
 constexpr int kRowWarps = 16, kMinRowWarps = 4;          // row kernel: warps per CTA
-constexpr int kRedoList = 512;                           // row kernel: blocks a CTA can leave for its float64 redo
 
 struct NormParams {
     nvfp4b_block_norm_args a;
@@ -525,7 +524,7 @@ struct Row64 {
     const void *y, *v;
     const uint4* w_post;
     int row, chunks;
-    bool has_v, g_col;
+    bool has_v, g_col, wild;
     double fgs, f, scale;
 
     __device__ __forceinline__ void r8(int ch, double (&r)[8]) const {
@@ -538,6 +537,9 @@ struct Row64 {
                 const V8 g = gate8(p, row, ch);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) r[k] = fma((double)n.at(k) * (double)w.at(k) * (double)g.at(k), fgs, r[k]);
+            } else if (Y == kBf16 && !wild) {                       // an exact fp32 product: one conversion for two
+#pragma unroll
+                for (int k = 0; k < 8; ++k) r[k] = fma((double)(n.at(k) * w.at(k)), fgs, r[k]);
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) r[k] = fma((double)n.at(k) * (double)w.at(k), fgs, r[k]);
@@ -563,9 +565,10 @@ struct Row64 {
         }
         return warp_sum(s);
     }
-    __device__ __forceinline__ Row64(const NormParams& p_, int row_, const void* y_, const void* v_, const uint4* w_post_)
+    __device__ __forceinline__ Row64(const NormParams& p_, int row_, const void* y_, const void* v_, const uint4* w_post_,
+                                     bool wild_)
         : p(p_), y(y_), v(v_), w_post(w_post_), row(row_), chunks(p_.a.H >> 3), has_v(p_.a.resid != nullptr),
-          scale((double)p_.a.scale) {
+          wild(wild_), scale((double)p_.a.scale) {
         const double h = (double)p.a.H, eps = (double)p.a.eps;
         g_col = Y != kNone && p.a.gate && p.a.gate_col_stride;
         fgs = scale * (Y != kNone && p.a.gate && !g_col ? (double)gate_at(p.a, row, 0) : 1.0);
@@ -581,7 +584,7 @@ __device__ __noinline__ uint32_t redo_row64(const NormParams& p, int row, uint32
                                             const void* v, const uint4* w_post, const uint4* w_norm) {
     const nvfp4b_block_norm_args& a = p.a;
     const int lane = threadIdx.x & 31;
-    const Row64<Y, R> q(p, row, y, v, w_post);
+    const Row64<Y, R> q(p, row, y, v, w_post, wild);
     __syncwarp();                                                   // codes and scale words stored before come first
     uint32_t zmax = 0;
     int step = 0;
@@ -635,9 +638,9 @@ __device__ __noinline__ uint32_t redo_row64(const NormParams& p, int row, uint32
 // z + d included) by
 //   d = f wm E T + Z E (1 + k),   E = 10 u,   k = sqrt(sum t^2 / sum r^2),   wm = max |norm_w|,
 // T = max |t| of the lane's chunks, Z = max |z| of the chunk (one d serves its 8 elements); without y by E |z|.  One row
-// in sixteen at 2816 elements holds an element that near to a border.  Those rows are listed and redone at the end, one
-// per warp at a time: redone on the spot, a row's float64 latency lands on one warp of the SM (76 against 51 us without
-// any redo).
+// in sixteen at 2816 elements holds an element that near to a border.  Its redo takes a warp nearly as long as the row
+// did, most of it conversions to float64, so the warps of a CTA take their rows from a common count (8192 x 2816 with a
+// gate: 55 us, 76 us with a fixed share of the rows for each warp).
 template <Src Y, Src R, bool MX>
 __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(const __grid_constant__ NormParams p) {
     using namespace sm100;
@@ -646,8 +649,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[kRowWarps];
     __shared__ uint32_t red_max[kRowWarps];
-    __shared__ int2 redo_list[kRedoList];                           // row, unproven block
-    __shared__ int listed, timeout;
+    __shared__ int taken, timeout;
     const nvfp4b_block_norm_args& a = p.a;
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5, chunks = a.H >> 3;
     const bool want_z = MX || a.out != nullptr;
@@ -667,8 +669,12 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
         if constexpr (HAS_Y) bulk_load(sy, y_row(row), yb, &full[wid]);
         if (rb) bulk_load(sr, v_row(row), rb, &full[wid]);
     };
-    const long long first = (long long)blockIdx.x * warps + wid, step = (long long)gridDim.x * warps;
-    if (threadIdx.x == 0) timeout = listed = 0;
+    // the CTA's rows: blockIdx.x + gridDim.x * (0, 1, 2 ...), the first `warps` of them by warp number, then as they come
+    const long long first = blockIdx.x + (long long)gridDim.x * wid;
+    if (threadIdx.x == 0) {
+        timeout = 0;
+        taken = warps;
+    }
     if (lane == 0) {
         mbar_init(&full[wid], 1);
         fence_mbar_init();
@@ -691,15 +697,17 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
     __syncthreads();                                                // red_max is used again at the end
 
     uint32_t zmax = 0, phase = 0;
-    for (long long lrow = first; lrow < a.T; lrow += step) {
+    for (long long lrow = first, next; lrow < a.T; lrow = next) {
         const int row = (int)lrow;
+        next = lane == 0 ? atomicAdd(&taken, 1) : 0;
+        next = blockIdx.x + (long long)gridDim.x * __shfl_sync(0xFFFFFFFFu, (int)next, 0);
         const float g_row = HAS_Y && a.gate && !a.gate_col_stride ? gate_at(a, row, 0) : 1.f;
         const bool g_col = HAS_Y && a.gate && a.gate_col_stride;
         mbar_wait(&full[wid], phase, &timeout, kErrTimeoutProducer);   // on expiry the kernel goes on and reports
         phase ^= 1u;
-        if (lane == 0 && lrow + step < a.T) {
-            if constexpr (HAS_Y) l2_prefetch(y_row(lrow + step), yb);
-            if (rb) l2_prefetch(v_row(lrow + step), rb);
+        if (lane == 0 && next < a.T) {
+            if constexpr (HAS_Y) l2_prefetch(y_row(next), yb);
+            if (rb) l2_prefetch(v_row(next), rb);
         }
         bool wild = false;
         float fgs = 1.f;                                            // scale * gate / rms(y)
@@ -837,12 +845,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
                     // also where the exponent is in doubt, or the values are near the ends of the range
                     const bool unsure = code != other || ((top ^ bot) & 0x7F800000u) != 0u ||
                                         top - 0x08800000u >= 0x7F000000u - 0x08800000u;
-                    if (unsure && top != 0u) {
-                        int slot = kRedoList;
-                        if (!later) slot = atomicAdd(&listed, 1);    // a block may be listed by each of its four lanes
-                        if (slot < kRedoList) redo_list[slot] = make_int2(row, ch >> 2);
-                        else doubt |= 1u << i;
-                    }
+                    doubt |= unsure && top != 0u ? 1u << i : 0u;
                     if (ok) code_row[ch] = code;
                     uint32_t w = ok ? ((field >> 23) - 2u) << (8 * ((lane & 15) >> 2)) : 0u;
                     w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
@@ -853,7 +856,20 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
         }
         doubt = __reduce_or_sync(0xFFFFFFFFu, doubt);               // from here on the same on every lane, as `wild` is
         if (wild || doubt != 0) {
-            const uint32_t m = redo_row64<Y, R, MX>(p, row, doubt, wild, y_row(row), a.resid ? v_row(row) : smem, w_post, w_norm);
+            const uint8_t *y = sy, *v = sr;
+            if (wild || !later) {                                   // r is not needed any more: the inputs once again
+                if constexpr (HAS_Y) {
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) fetch(row);
+                    mbar_wait(&full[wid], phase, &timeout, kErrTimeoutProducer);
+                    phase ^= 1u;
+                }
+            } else {
+                if constexpr (HAS_Y) y = y_row(row);
+                v = a.resid ? v_row(row) : smem;
+            }
+            const uint32_t m = redo_row64<Y, R, MX>(p, row, doubt, wild, y, v, w_post, w_norm);
             row_max = wild ? m : row_max;
         }
         if (later && !wild) {
@@ -867,21 +883,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
         zmax = max(zmax, row_max);
         fence_proxy_async();                                        // r's writes before the copies' ones
         __syncwarp();                                               // every lane is done with the buffer
-        if (lane == 0 && lrow + step < a.T) fetch(lrow + step);
+        if (lane == 0 && next < a.T) fetch(next);
     }
 
-    if constexpr (MX) {
-        zero_padding_rows(p);
-        __syncthreads();
-        for (int i = wid; i < min(listed, kRedoList); i += warps) {
-            const int2 e = redo_list[i];
-            if (lane == 0) fetch(e.x);
-            mbar_wait(&full[wid], phase, &timeout, kErrTimeoutProducer);
-            phase ^= 1u;
-            redo_row64<Y, R, true>(p, e.x, 1u << (e.y >> 3), false, sy, sr, w_post, w_norm);
-            __syncwarp();                                           // every lane is done with the buffer
-        }
-    }
+    if constexpr (MX) zero_padding_rows(p);
     if (a.amax) {
         zmax = __reduce_max_sync(0xFFFFFFFFu, zmax);
         if (lane == 0) red_max[wid] = zmax;
@@ -918,18 +923,10 @@ int launch_block_norm_rows(NormParams& p, cudaStream_t s, bool& fits) {
     fits = warps >= kMinRowWarps && p.a.H <= 32 * 256;
     if (!fits) return NVFP4B_OK;
     if (warps > kRowWarps) warps = kRowWarps;
-    // the count of warps whose last round of rows leaves the fewest idle
-    const int sms = sm_count();
-    long long best = -1;
-    for (int w = warps, most = warps; w >= most - most / 4; --w) {
-        const long long rounds = (p.a.T + (long long)sms * w - 1) / ((long long)sms * w) * w;
-        if (best < 0 || rounds < best) { best = rounds; warps = w; }
-    }
     static std::atomic<bool> ready[64];
     const int st = raise_smem(reinterpret_cast<const void*>(kernel), ready);
     if (st) return st;
-    long long grid = ((long long)p.a.T + warps - 1) / warps;
-    if (grid > sms) grid = sms;
+    const int grid = p.a.T < sm_count() ? p.a.T : sm_count();       // rows dealt over every SM first
     return launch_k(kernel, dim3((unsigned)grid), dim3(warps * 32), p.weight_bytes + warps * p.stage_bytes, s, p);
 }
 
@@ -955,9 +952,11 @@ int launch_block_norm(NormParams& p, cudaStream_t s) {
     return launch_k(kernel, dim3((unsigned)grid), dim3(threads), smem, s, p);
 }
 
-// A CTA per row, one chunk per thread where that fits (four above 4096 elements); from kRowKernelRows rows per SM on, a
-// warp per row, where its rings fit (rows of up to 24 KB of input).
-constexpr int kRowKernelRows = 8;
+// From kRowKernelRows rows per SM on a warp per row, where its buffers fit (800 x 2816 fp32 to bf16 9 us, 10 by CTAs; 512
+// rows 7.5 and 6.9).  Below a CTA per row: one chunk per thread, the shortest path through a row, as far as the rows make
+// two rounds (64 x 2816 with y to MXFP4 6.2 us; 512 x 704 3.4 us, 4.7 with four); else four chunks, for more CTAs per SM
+// (512 x 2816 with y to MXFP4 11.8 us, 14.5 with one).
+constexpr int kRowKernelRows = 5;
 
 template <Src Y, Src R>
 int dispatch_block_norm(NormParams& p, cudaStream_t s) {   // R = kBf16 without resid
@@ -967,7 +966,8 @@ int dispatch_block_norm(NormParams& p, cudaStream_t s) {   // R = kBf16 without 
                                  : launch_block_norm_rows<Y, R, false>(p, s, fits);
         if (fits) return st;
     }
-    const bool wide = p.a.H <= 8 * kNormMaxThreads;
+    const int chunks = p.a.H / 8, resident = kNormMaxThreads / ((chunks + 31) / 32 * 32);    // CTAs per SM, one chunk each
+    const bool wide = resident >= 1 && p.a.T <= 2 * sm_count() * resident;
     if (p.a.codes) return wide ? launch_block_norm<Y, R, 1, true>(p, s) : launch_block_norm<Y, R, 4, true>(p, s);
     return wide ? launch_block_norm<Y, R, 1, false>(p, s) : launch_block_norm<Y, R, 4, false>(p, s);
 }
