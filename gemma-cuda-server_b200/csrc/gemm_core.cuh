@@ -70,6 +70,7 @@ struct KCfg {
     static_assert(SF_COL0 + SF_SLOTS * (SF_COLS_A + SF_COLS_B) <= TMEM_COLS, "TMEM budget");
     static_assert(SMEM_BYTES <= 232448, "shared memory budget");
     static_assert(BN % 128 == 0 && BN <= 256, "BN");
+    static_assert(KIND != Kind::MXF4, "the MXFP4 GEMM has its own single-CTA kernel");
     static_assert(EPI_WARPS == 4 || EPI_WARPS == 8, "epilogue warps");
     static_assert(COLS_PER_WARP % 32 == 0, "chunking");
 };
@@ -348,9 +349,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             const uint64_t a_desc = desc_kmajor_sw128(smem_u32(sA)), b_desc = desc_kmajor_sw128(smem_u32(sB));
             for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
                 const TileInfo ti = sched.tile(t);
-                const uint32_t idesc = C::KIND == Kind::NVF4   ? idesc_nvf4(C::BM, ti.n_mma)
-                                       : C::KIND == Kind::MXF4 ? idesc_mxf4(C::BM, ti.n_mma)
-                                                               : idesc_bf16(C::BM, ti.n_mma);
+                const uint32_t idesc = C::SCALED ? idesc_nvf4(C::BM, ti.n_mma) : idesc_bf16(C::BM, ti.n_mma);
                 if (!mbar_wait(&tempty[abuf], aphase ^ 1u, sflag, kErrTimeoutMma)) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem + (uint32_t)(abuf * C::BN);

@@ -35,11 +35,6 @@ __device__ __forceinline__ size_t mx_scale_offset(int m, int b, int tile_cols) {
     return ((size_t)(m >> 7) * tile_cols + (b >> 2)) * 512 + (m & 31) * 16 + ((m & 127) >> 5) * 4 + (b & 3);
 }
 
-// Codes of 8 elements, element 0 in the lowest nibble.
-__device__ __forceinline__ uint32_t mx_encode8(const float* v, float inv) {
-    return cvt_e2m1x8(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-}
-
 // Scale byte of a float64 block maximum.
 __device__ __forceinline__ uint32_t mx_byte64(double amax) {
     if (!(amax < 3.402823669209384634634e38)) return 255u;       // 2^128 and more, infinities, NaN

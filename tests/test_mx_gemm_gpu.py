@@ -48,6 +48,8 @@ SIZES = [(1, 1, 32), (1, 2816, 2816), (2, 129, 64), (3, 4224, 96), (8, 130, 2112
          (17, 257, 288), (31, 704, 2816), (33, 96, 1056), (64, 2816, 704), (65, 500, 352), (100, 8448, 2816),
          (127, 255, 480), (128, 512, 4096), (129, 129, 32), (200, 333, 2848), (256, 256, 256), (257, 700, 544),
          (333, 2001, 1056), (512, 2816, 2112), (640, 1, 320)]
+# More than 128 rows and more 128 x 128 tiles than SMs: tiles of CTA pairs, up to several a pair.
+SIZES += [(129, 19001, 96), (1281, 2001, 160), (2050, 1304, 288), (19100, 1, 64), (1000, 5000, 2848), (4200, 3001, 480)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
@@ -59,7 +61,7 @@ def test_gemm_vs_float64(m, n, k, kind):
     _close(got, mx.dequantize(*a), mx.dequantize(*b), k, 2.0 ** -8 if kind == "bf16" else 2.0 ** -24)
 
 
-@pytest.mark.parametrize("m,n,k", [(5, 300, 416), (200, 300, 416)])
+@pytest.mark.parametrize("m,n,k", [(5, 300, 416), (200, 300, 416), (1500, 1804, 416)])
 def test_alpha_and_strided_output(m, n, k):
     p = require_gpu()
     a, b = _operand(m, k, 3), _operand(n, k, 4)
@@ -73,7 +75,7 @@ def test_alpha_and_strided_output(m, n, k):
             assert (wide[:, c:] == 5.0).all()
 
 
-@pytest.mark.parametrize("m,n,k", [(3, 200, 96), (40, 200, 96), (300, 200, 96)])
+@pytest.mark.parametrize("m,n,k", [(3, 200, 96), (40, 200, 96), (300, 200, 96), (1700, 1500, 96)])
 def test_scale_bytes_over_their_range(m, n, k):
     """Every exponent from the smallest to large ones, opposite in A and B so that the products stay in range; a NaN scale
     makes exactly its row or column NaN."""
@@ -97,7 +99,7 @@ def test_scale_bytes_over_their_range(m, n, k):
 def test_same_bits_every_time_and_for_every_row_count():
     """Two calls give the same bits, and so do two graph replays on fresh contents of the same buffers."""
     p = require_gpu()
-    for m, n, k in [(1, 2816, 2816), (16, 4224, 2816), (300, 1000, 1056)]:
+    for m, n, k in [(1, 2816, 2816), (16, 4224, 2816), (300, 1000, 1056), (1300, 4001, 1056)]:
         a, b = _dev(*_operand(m, k, 7), k), _dev(*_operand(n, k, 8), k)
         one = p.mx_gemm(*a, *b, out_kind=p.OUT_F32_ROWMAJOR)
         assert torch.equal(one, p.mx_gemm(*a, *b, out_kind=p.OUT_F32_ROWMAJOR))
