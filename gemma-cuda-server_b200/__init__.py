@@ -465,8 +465,8 @@ def block_norm(resid: torch.Tensor | None = None, norm_weight: torch.Tensor | No
     resid, y: bf16 or fp32 [T, H] (either may be None); the weights bf16 [H] (None = ones); post_norm: whether y is
     normalised (default: with a post_weight); gate: bf16 or fp32, [H] per feature, [T, 1] per token or [T, H].
     z goes to `out` (bf16 [T, H]; with `amax`, fp32 [1], its max |z|) and / or to MXFP4 `codes` and `scales` (mx=True
-    allocates them).  Without any of these, z is written to a new `out` if norm_weight is given, and r to a new
-    resid_out (of resid's type, or y's) if y is.  resid_out may be resid itself."""
+    allocates them); with a norm_weight and neither, to a new `out`.  Where nothing is asked for but y is given, r goes to
+    a new resid_out of resid's type (or y's).  resid_out and out may be resid or y themselves, of the same type and pitch."""
     x = resid if resid is not None else y
     if x is None:
         raise ValueError("block_norm: resid or y is needed")
@@ -514,11 +514,6 @@ def block_norm(resid: torch.Tensor | None = None, norm_weight: torch.Tensor | No
     if out is not None:
         a.ld_out = _rows("block_norm: out", out, (torch.bfloat16,), (T, H), dev)
         a.out = out.data_ptr()
-        for t, ld in ((resid, a.ld_resid), (y, a.ld_y)):
-            if t is not None and a.out == t.data_ptr() and (out.dtype, a.ld_out) != (t.dtype, ld):
-                raise ValueError("block_norm: out on an input of another type or pitch")
-        if resid_out is not None and a.out == a.resid_out:
-            raise ValueError("block_norm: out on resid_out")
     if amax is not None:
         if out is None:
             raise ValueError("block_norm: amax needs out")

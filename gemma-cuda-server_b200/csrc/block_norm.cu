@@ -974,6 +974,35 @@ int dispatch_block_norm(NormParams& p, cudaStream_t s) {   // R = kBf16 without 
 
 bool bad_rows(const void* p, int f32, long long ld) { return !aligned16(p) || (ld * (f32 ? 4 : 2)) % 16; }
 
+// T rows of `width` bytes, `pitch` bytes apart (p NULL: not there).
+struct Region {
+    const void* p;
+    long long pitch, width;
+};
+
+// Whether two regions share memory otherwise than row for row (`same` allowed) -- side by side in the same pitch they do not.
+bool clash(const Region& a, const Region& b, long long T, bool same) {
+    if (!a.p || !b.p) return false;
+    const long long pa = (long long)reinterpret_cast<uintptr_t>(a.p), pb = (long long)reinterpret_cast<uintptr_t>(b.p);
+    if (pa >= pb + (T - 1) * b.pitch + b.width || pb >= pa + (T - 1) * a.pitch + a.width) return false;
+    if (same && pa == pb && a.width == b.width && (T == 1 || a.pitch == b.pitch)) return false;
+    if (a.pitch != b.pitch || a.pitch <= 0) return true;
+    const long long d = ((pb - pa) % a.pitch + a.pitch) % a.pitch;
+    return d < a.width || d + b.width > a.pitch;
+}
+
+bool clashes(const nvfp4b_block_norm_args& a) {
+    const auto rows = [&](const void* p, int f32, long long ld) { return Region{p, ld * (f32 ? 4 : 2), a.H * (f32 ? 4ll : 2ll)}; };
+    const Region in[] = {rows(a.resid, a.resid_f32, a.ld_resid), rows(a.y, a.y_f32, a.ld_y)};
+    const Region r = rows(a.resid_out, a.resid_out_f32, a.ld_resid_out), z = rows(a.out, 0, a.ld_out);
+    const Region c = {a.codes, a.H / 2, a.H / 2};
+    const Region g = a.gate_col_stride ? rows(a.gate, a.gate_f32, a.gate_row_stride) : Region{};
+    for (const Region& x : in)
+        if (clash(r, x, a.T, true) || clash(z, x, a.T, true) || clash(c, x, a.T, false)) return true;
+    return clash(r, z, a.T, false) || clash(r, c, a.T, false) || clash(z, c, a.T, false) || clash(r, g, a.T, false) ||
+           clash(z, g, a.T, false) || clash(c, g, a.T, false);
+}
+
 }  // namespace
 }  // namespace nvfp4b
 
@@ -1000,6 +1029,7 @@ extern "C" int nvfp4b_block_norm(const nvfp4b_block_norm_args* args, void* strea
         !aligned16(a.codes) || !aligned16(a.scales) || (reinterpret_cast<uintptr_t>(a.gate) & (a.gate_f32 ? 3 : 1)) ||
         (reinterpret_cast<uintptr_t>(a.amax) & 3))
         return NVFP4B_ERR_ALIGN;
+    if (clashes(a)) return NVFP4B_ERR_ARG;
     const cudaStream_t s = (cudaStream_t)stream;
     if (a.amax) {
         const cudaError_t e = cudaMemsetAsync(a.amax, 0, sizeof(float), s);

@@ -372,7 +372,7 @@ extern "C" int nvfp4b_mx_quantize_f32(const float* x, long long ldx, int M, int 
 
 extern "C" int nvfp4b_mx_geglu_quantize(const void* gate_up, long long ld, int M, int I, uint8_t* codes,
                                         uint8_t* scales, void* stream) {
-    if (I > (1 << 30)) return NVFP4B_ERR_SHAPE;
+    if (I >= (1 << 30)) return NVFP4B_ERR_SHAPE;
     const int st = mx_check(gate_up, codes, scales, ld, M, I, 2 * I, 2);
     if (st) return st;
     MxGrid g;

@@ -208,6 +208,42 @@ def test_in_place_strided_and_defaults():
     assert only_z.resid is None and torch.equal(only_z.out, got.out)
 
 
+@pytest.mark.parametrize("T", [50, 1300])
+@pytest.mark.parametrize("dtype", [B, F])
+def test_in_place_equals_apart(T, dtype):
+    """Outputs on the inputs, and beside them in one buffer, give the bits that separate ones do."""
+    p = require_gpu()
+    base = _make(T, 512, 12, dtype, B, gate="row")
+    new = lambda t: torch.empty_like(t)  # noqa: E731
+    for mx_too in (False, True):
+        want = p.block_norm(**base, resid_out=new(base["resid"]), out=new(base["y"]), mx=mx_too)
+        kw = {**base, "resid": base["resid"].clone(), "y": base["y"].clone()}
+        got = p.block_norm(**kw, resid_out=kw["resid"], out=kw["y"], mx=mx_too)
+        assert torch.equal(got.resid, want.resid) and torch.equal(got.out, want.out)
+        if mx_too:
+            assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+    wide = torch.empty(T, 1024, dtype=dtype, device="cuda")
+    wide[:, 512:] = base["resid"]
+    got = p.block_norm(**{**base, "resid": wide[:, 512:]}, resid_out=wide[:, :512], mx=True)
+    assert torch.equal(got.resid, want.resid) and torch.equal(got.codes, want.codes)
+    assert torch.equal(wide[:, 512:], base["resid"])
+    with pytest.raises(p.NvFp4Error, match="ARG"):
+        p.block_norm(wide[1:, :512], base["norm_weight"], resid_out=wide[:-1, :512])
+
+
+def test_two_streams_at_once():
+    p = require_gpu()
+    for T in (3, 1300):
+        kw = [_make(T, 2816, 20 + i, F, B, gate="row") for i in range(2)]
+        want = [p.block_norm(mx=True, **k) for k in kw]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in kw]
+        got = [[p.block_norm(mx=True, stream=s, **k) for _ in range(8)] for k, s in zip(kw, streams)]
+        torch.cuda.synchronize()
+        for gs, w in zip(got, want):
+            assert all(torch.equal(g.codes, w.codes) and torch.equal(g.scales, w.scales) for g in gs)
+
+
 def test_amax_feeds_the_nvfp4_quantiser():
     p = require_gpu()
     kw = _make(200, 704, 10, F, F)

@@ -103,3 +103,27 @@ def test_block_norm_c_refusals():
     assert call(resid=8) == -2 and call(ld_resid=68) == -2 and call(norm_weight=8, out=16, ld_out=64) == -2
     assert call(y=16, ld_y=64, gate=18, gate_f32=1) == -2
     assert call(out=16, ld_out=64, amax=18) == -2
+
+
+def test_block_norm_refuses_rows_that_share_memory():
+    """Rows of 64 bf16 (128 bytes) at made-up addresses; what is allowed launches, and is tested on the GPU."""
+    p = load_package()
+    L, A = p._mx_sigs(), p._BlockNormArgs
+    base = 1 << 20
+
+    def call(**kw):
+        kw = {**dict(T=4, H=64, resid=base, ld_resid=64, eps=1e-6, scale=1.0), **kw}
+        return L.nvfp4b_block_norm(A(**kw), None)
+
+    far = base + (1 << 16)
+    assert call(resid_out=base + 128, ld_resid_out=64) == -7                          # a row further on
+    assert call(resid_out=base, ld_resid_out=72) == -7                                # another pitch
+    assert call(resid_out=base, ld_resid_out=64, resid_out_f32=1) == -7               # another type
+    assert call(resid_out=base - 512 + 16, ld_resid_out=64) == -7                     # the last row reaches in
+    assert call(ld_resid=128, resid_out=base + 64, ld_resid_out=128) == -7            # half a row aside
+    assert call(ld_resid=128, resid_out=base + 192, ld_resid_out=128) == -7           # wraps into the next row
+    assert call(y=far, ld_y=64, out=far + 128, ld_out=64) == -7
+    assert call(y=far, ld_y=64, y_f32=1, out=far, ld_out=64) == -7
+    assert call(resid_out=far, ld_resid_out=64, out=far, ld_out=64) == -7             # two outputs
+    assert call(codes=base + 256, scales=far) == -7
+    assert call(y=far, ld_y=64, gate=far + 4096, gate_row_stride=64, gate_col_stride=1, out=far + 4096, ld_out=64) == -7
