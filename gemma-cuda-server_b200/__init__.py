@@ -18,6 +18,7 @@ Two layers:
 from __future__ import annotations
 
 import ctypes
+import functools
 import pathlib
 from typing import NamedTuple
 
@@ -251,10 +252,9 @@ class _BlockNormArgs(ctypes.Structure):
                 ("amax", _P), ("codes", _P), ("scales", _P)]
 
 
+@functools.cache
 def _mx_sigs():
     L = lib()
-    if getattr(L, "_mx_ready", False):
-        return L
     ll = ctypes.c_longlong
     sig = {
         "nvfp4b_mx_scale_buffer_bytes": ([ctypes.c_int, ctypes.c_int], ctypes.c_size_t),
@@ -271,7 +271,6 @@ def _mx_sigs():
         f = getattr(L, name)
         f.argtypes = args
         f.restype = res
-    L._mx_ready = True
     return L
 
 
@@ -296,21 +295,21 @@ def _rows(name: str, t: torch.Tensor, dtypes, shape, device: int | None = None) 
     return pitch
 
 
-def _flat(name: str, t: torch.Tensor, dtype, numel: int, device: int) -> None:
+def _flat(name: str, t: torch.Tensor, dtype, numel: int, device: int, part: str = "") -> None:
     """Checks a contiguous tensor of at least `numel` elements on a CUDA device."""
     if t.dtype != dtype or t.numel() < numel or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{name}: needs {numel} contiguous {dtype} elements on cuda:{device}, got {t.numel()} of "
+        raise ValueError(f"{name}{part}: needs {numel} contiguous {dtype} elements on cuda:{device}, got {t.numel()} of "
                          f"{t.dtype} on {t.device}")
 
 
-def _empty(shape, dtype, device: int, stream) -> torch.Tensor:
-    device = torch.device("cuda", device)
+def _empty(like: torch.Tensor, shape, dtype, stream) -> torch.Tensor:
+    """New tensor on `like`'s device, allocated on the stream of the call."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
     if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device)
+        stream = torch.cuda.ExternalStream(stream, device=like.device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
 
 
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
@@ -347,7 +346,7 @@ def mx_swizzle_scales(logical: torch.Tensor, outer: int, K: int, stream=None) ->
         raise ValueError(f"mx_swizzle_scales: logical: on {logical.device}, expected a CUDA device")
     dev = logical.get_device()
     _flat("mx_swizzle_scales: logical", logical, torch.uint8, outer * (K // 32), dev)
-    out = _empty(mx_scale_buffer_bytes(outer, K), torch.uint8, dev, stream)
+    out = _empty(logical, mx_scale_buffer_bytes(outer, K), torch.uint8, stream)
     _launch("mx_swizzle_scales", _mx_sigs().nvfp4b_mx_swizzle_scales, dev, stream, logical.data_ptr(),
             out.data_ptr(), outer, K)
     return out
@@ -365,21 +364,23 @@ def _mx_operand(name: str, codes: torch.Tensor, scales: torch.Tensor, device: in
         device = codes.get_device()
         if device < 0:
             raise ValueError(f"{name}: on {codes.device}, expected a CUDA device")
-    _mx_buffers(name, M, 2 * half, codes, scales, device, None)
+    _mx_buffers(name, M, 2 * half, codes, scales, device)
     return M, 2 * half, device
 
 
-def _mx_buffers(name: str, M: int, K: int, codes, scales, device: int, stream):
+def _mx_buffers(name: str, M: int, K: int, codes, scales, device: int, like=None, stream=None):
+    """Checks the codes and scales of an [M, K] operand; what is None is allocated, as `_empty` does."""
     if K % 32:
         raise ValueError(f"{name}: width {K} is not a multiple of 32")
+    n = mx_scale_buffer_bytes(M, K)
     if codes is None:
-        codes = _empty((M, K // 2), torch.uint8, device, stream)
+        codes = _empty(like, (M, K // 2), torch.uint8, stream)
     else:
-        _flat(name + ": codes", codes, torch.uint8, M * (K // 2), device)
+        _flat(name, codes, torch.uint8, M * (K // 2), device, ": codes")
     if scales is None:
-        scales = _empty(mx_scale_buffer_bytes(M, K), torch.uint8, device, stream)
+        scales = _empty(like, n, torch.uint8, stream)
     else:
-        _flat(name + ": scales", scales, torch.uint8, mx_scale_buffer_bytes(M, K), device)
+        _flat(name, scales, torch.uint8, n, device, ": scales")
     return codes, scales
 
 
@@ -389,7 +390,7 @@ def mx_quantize(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torc
     ld = _rows("mx_quantize: x", x, (torch.bfloat16, torch.float32), (None, None))
     M, K = x.shape
     dev = x.get_device()
-    codes, scales = _mx_buffers("mx_quantize", M, K, codes, scales, dev, stream)
+    codes, scales = _mx_buffers("mx_quantize", M, K, codes, scales, dev, x, stream)
     L = _mx_sigs()
     fn = L.nvfp4b_mx_quantize_bf16 if x.dtype == torch.bfloat16 else L.nvfp4b_mx_quantize_f32
     _launch("mx_quantize", fn, dev, stream, x.data_ptr(), ld, M, K, codes.data_ptr(), scales.data_ptr())
@@ -405,7 +406,7 @@ def mx_geglu_quantize(gate_up: torch.Tensor, codes: torch.Tensor | None = None, 
     if gate_up.shape[1] % 2:
         raise ValueError("mx_geglu_quantize: odd width")
     dev = gate_up.get_device()
-    codes, scales = _mx_buffers("mx_geglu_quantize", M, I, codes, scales, dev, stream)
+    codes, scales = _mx_buffers("mx_geglu_quantize", M, I, codes, scales, dev, gate_up, stream)
     _launch("mx_geglu_quantize", _mx_sigs().nvfp4b_mx_geglu_quantize, dev, stream, gate_up.data_ptr(), ld, M, I,
             codes.data_ptr(), scales.data_ptr())
     return codes, scales
@@ -416,7 +417,7 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype 
     """The values of MXFP4 codes [M, K/2] and tile-layout scales as bf16 or fp32 [M, K] (exact in both)."""
     M, K, dev = _mx_operand("mx_dequantize", codes, scales)
     if out is None:
-        out = _empty((M, K), dtype, dev, stream)
+        out = _empty(codes, (M, K), dtype, stream)
     ld = _rows("mx_dequantize: out", out, _FLOATS, (M, K), dev)
     _launch("mx_dequantize", _mx_sigs().nvfp4b_mx_dequantize, dev, stream, codes.data_ptr(), scales.data_ptr(), M, K,
             out.data_ptr(), 1 if out.dtype == torch.float32 else 0, ld)
@@ -437,7 +438,7 @@ def mx_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: 
     shape = (N, M) if out_kind == OUT_F32_COLMAJOR else (M, N)
     dtype = torch.bfloat16 if out_kind == OUT_BF16_ROWMAJOR else torch.float32
     if out is None:
-        out = _empty(shape, dtype, dev, stream)
+        out = _empty(a, shape, dtype, stream)
     ldd = _rows("mx_gemm: out", out, (dtype,), shape, dev)
     _launch("mx_gemm", _mx_sigs().nvfp4b_mx_gemm, dev, stream, a.data_ptr(), a_scales.data_ptr(), b.data_ptr(),
             b_scales.data_ptr(), float(alpha), M, N, K, out.data_ptr(), out_kind, ldd)
@@ -485,7 +486,7 @@ def block_norm(resid: torch.Tensor | None = None, norm_weight: torch.Tensor | No
         a.ld_y = _rows("block_norm: y", y, _FLOATS, (T, H), dev)
         a.y, a.y_f32 = y.data_ptr(), y.dtype == torch.float32
         if resid_out is None and out is None and not mx and norm_weight is None:
-            resid_out = _empty((T, H), x.dtype, dev, stream)
+            resid_out = _empty(x, (T, H), x.dtype, stream)
     elif post_weight is not None or post_norm or gate is not None:
         raise ValueError("block_norm: post_weight, post_norm and gate need y")
     if post_weight is not None:
@@ -505,7 +506,7 @@ def block_norm(resid: torch.Tensor | None = None, norm_weight: torch.Tensor | No
         _flat("block_norm: norm_weight", norm_weight, torch.bfloat16, H, dev)
         a.norm_weight = norm_weight.data_ptr()
         if out is None and not mx:
-            out = _empty((T, H), torch.bfloat16, dev, stream)
+            out = _empty(x, (T, H), torch.bfloat16, stream)
     if resid_out is not None:
         a.ld_resid_out = _rows("block_norm: resid_out", resid_out, _FLOATS, (T, H), dev)
         a.resid_out, a.resid_out_f32 = resid_out.data_ptr(), resid_out.dtype == torch.float32
@@ -520,7 +521,7 @@ def block_norm(resid: torch.Tensor | None = None, norm_weight: torch.Tensor | No
         _flat("block_norm: amax", amax, torch.float32, 1, dev)
         a.amax = amax.data_ptr()
     if mx:
-        codes, scales = _mx_buffers("block_norm", T, H, codes, scales, dev, stream)
+        codes, scales = _mx_buffers("block_norm", T, H, codes, scales, dev, x, stream)
         a.codes, a.scales = codes.data_ptr(), scales.data_ptr()
     _launch("block_norm", _mx_sigs().nvfp4b_block_norm, dev, stream, ctypes.byref(a))
     return BlockNorm(resid_out, out, amax, codes, scales)
