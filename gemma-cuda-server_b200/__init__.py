@@ -275,14 +275,14 @@ def _mx_sigs():
 
 
 def _rows(name: str, t: torch.Tensor, dtypes, shape, device: int | None = None) -> int:
-    """Checks a [rows, columns] CUDA tensor with unit column stride; returns its row pitch in elements.  None in
-    `shape` stands for any size, None for the device index for any CUDA device."""
-    got = t.shape
+    """Checks a [rows, columns] CUDA tensor with unit column stride; returns its row pitch in elements.  None for
+    `shape` stands for any, None for the device index for any CUDA device."""
+    got, dev = t.shape, t.get_device()
     if t.dtype not in dtypes:
         raise ValueError(f"{name}: dtype {t.dtype}, expected one of {dtypes}")
-    if len(got) != 2 or (shape[0] is not None and shape[0] != got[0]) or (shape[1] is not None and shape[1] != got[1]):
-        raise ValueError(f"{name}: shape {tuple(got)}, expected {tuple(shape)}")
-    if not t.is_cuda or (device is not None and t.get_device() != device):
+    if len(got) != 2 or (shape is not None and shape != got):
+        raise ValueError(f"{name}: shape {tuple(got)}, expected {'[rows, columns]' if shape is None else tuple(shape)}")
+    if dev < 0 or (device is not None and dev != device):
         raise ValueError(f"{name}: on {t.device}, expected {'a CUDA device' if device is None else f'cuda:{device}'}")
     rows, cols = got
     pitch, unit = t.stride()
@@ -352,20 +352,22 @@ def mx_swizzle_scales(logical: torch.Tensor, outer: int, K: int, stream=None) ->
     return out
 
 
-_FLOATS = (torch.bfloat16, torch.float32)
+_FLOATS, _U8 = (torch.bfloat16, torch.float32), torch.uint8
 
 
 def _mx_operand(name: str, codes: torch.Tensor, scales: torch.Tensor, device: int | None = None):
     """Checks MXFP4 codes [rows, K/2] with their tile-layout scales; returns rows, K and the device index."""
-    if codes.dim() != 2:
-        raise ValueError(f"{name}: shape {tuple(codes.shape)}, expected [rows, K/2]")
-    M, half = codes.shape
-    if device is None:
-        device = codes.get_device()
-        if device < 0:
-            raise ValueError(f"{name}: on {codes.device}, expected a CUDA device")
-    _mx_buffers(name, M, 2 * half, codes, scales, device)
-    return M, 2 * half, device
+    shape, dev = codes.shape, codes.get_device()
+    if len(shape) != 2:
+        raise ValueError(f"{name}: shape {tuple(shape)}, expected [rows, K/2]")
+    if dev < 0 or (device is not None and dev != device):
+        raise ValueError(f"{name}: on {codes.device}, expected {'a CUDA device' if device is None else f'cuda:{device}'}")
+    M, half = shape
+    if (half & 15 or codes.dtype is not _U8 or scales.dtype is not _U8 or scales.get_device() != dev or
+            not codes.is_contiguous() or not scales.is_contiguous() or
+            scales.numel() < (M + 127 >> 7) * (half + 63 >> 6) * 512):
+        _mx_buffers(name, M, 2 * half, codes, scales, dev)         # raises, with the reason
+    return M, 2 * half, dev
 
 
 def _mx_buffers(name: str, M: int, K: int, codes, scales, device: int, like=None, stream=None):
@@ -387,7 +389,7 @@ def _mx_buffers(name: str, M: int, K: int, codes, scales, device: int, like=None
 def mx_quantize(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None, stream=None):
     """MXFP4-quantise a bf16 or fp32 [M, K] device tensor (K % 32 == 0; rows may be strided, with a row pitch of a
     multiple of 16 bytes).  Returns (codes [M, K/2] uint8, tile-layout e8m0 scales uint8)."""
-    ld = _rows("mx_quantize: x", x, (torch.bfloat16, torch.float32), (None, None))
+    ld = _rows("mx_quantize: x", x, _FLOATS, None)
     M, K = x.shape
     dev = x.get_device()
     codes, scales = _mx_buffers("mx_quantize", M, K, codes, scales, dev, x, stream)
@@ -401,7 +403,7 @@ def mx_geglu_quantize(gate_up: torch.Tensor, codes: torch.Tensor | None = None, 
                       stream=None):
     """gelu_tanh(gate) * up of bf16 rows [gate (I) | up (I)], quantised to MXFP4 (the codes of the float64 value).
     Returns (codes [M, I/2] uint8, tile-layout e8m0 scales uint8), the second product's A operand."""
-    ld = _rows("mx_geglu_quantize: gate_up", gate_up, (torch.bfloat16,), (None, None))
+    ld = _rows("mx_geglu_quantize: gate_up", gate_up, (torch.bfloat16,), None)
     M, I = gate_up.shape[0], gate_up.shape[1] // 2
     if gate_up.shape[1] % 2:
         raise ValueError("mx_geglu_quantize: odd width")

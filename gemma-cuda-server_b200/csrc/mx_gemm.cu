@@ -387,6 +387,7 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 1)
             if (buf == 0) aphase ^= 1u;
         }
     }
+    __syncwarp();
     if (S > 1) {                                                  // one tile per cluster
         cluster_sync();
         const int nb = t0 / p.m_tiles, mb = t0 - nb * p.m_tiles;
