@@ -3,6 +3,10 @@
 Tolerance: the output rounding (half a step: 2^-8 bf16, 2^-24 fp32, relative) plus fp32 accumulation -- every 64-element
 MMA step rounds its own sum and the running sum, each by at most 2^-23 of S = sum |a b| (truncation), so
 2 (steps + 1) 2^-23 S in all, plus the joins of a split K, at most 8 more."""
+import pathlib
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -111,6 +115,36 @@ def test_same_bits_every_time_and_for_every_row_count():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, one)
+
+
+FIRST_CALLS = """
+import torch
+from __graft_entry__ import load_package
+p = load_package()
+x = torch.randn(64, 704, device="cuda").bfloat16()
+ones = torch.ones(704, device="cuda").bfloat16()
+u8 = lambda n, v: torch.full((n,), v, dtype=torch.uint8, device="cuda")
+a, b = u8(16 * 352, 0x21).view(16, 352), u8(2048 * 352, 0x42).view(2048, 352)
+sa, sb = u8(p.mx_scale_buffer_bytes(16, 704), 127), u8(p.mx_scale_buffer_bytes(2048, 704), 127)
+calls = [lambda: p.mx_quantize(x), lambda: p.mx_geglu_quantize(x), lambda: p.mx_dequantize(a, sa),
+         lambda: p.mx_gemm(a, sa, b, sb), lambda: p.mx_gemm(b, sb, b, sb), lambda: p.block_norm(x, ones, mx=True)]
+for call in calls:
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = call()
+    graph.replay()
+    want = call()
+    for g, w in zip(*[r if isinstance(r, tuple) else (r,) for r in (got, want)]):
+        assert g is None or torch.equal(g.view(torch.uint8), w.view(torch.uint8))
+assert p.read_device_error() == 0
+"""
+
+
+def test_first_calls_may_be_captured():
+    """A process whose first call of each entry is captured: nothing is set up that a capture forbids."""
+    require_gpu()
+    subprocess.run([sys.executable, "-c", FIRST_CALLS], check=True, cwd=pathlib.Path(__file__).parents[1], timeout=120)
 
 
 def test_two_streams_at_once():
