@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "gemm_core.cuh"
@@ -138,20 +139,22 @@ int mx_core_params(const MxGemm& g, CoreParams& cp) {
 // about 200 KB of stages; persistent over tiles when S = 1, with two accumulators.
 //   warp 0      producer: TMA loads of the weights (128 x 128 bytes) and of A (NT x 128 bytes), bulk loads of the scales
 //   warp 1      TMEM owner and MMA issuer
-//   warps 2-5   epilogue, TMEM lane quadrant warp % 4: a thread holds one column n of D for all rows of the tile; 16 rows
-//               at a time are turned around in shared memory so that a lane stores 16 bytes
-//   warp 6      scale copies (issued by the MMA thread they made a K-tile take 1330 cycles)
+//   warps 2..   epilogue, TMEM lane quadrant warp % 4: a thread holds one column n of D, 16 rows at a time.  Eight warps from
+//               32 rows on, two to a quadrant: a warp's own instructions are what the epilogue takes (512 x 2816,
+//               K = 2112 8.9 us with four, 8.4 with eight, no gain with sixteen)
+//   last warp   scale copies (issued by the MMA thread they made a K-tile take 1330 cycles)
 template <int NT_>
 struct SkinnyCfg {
     static constexpr int NT = NT_, A_BYTES = NT * 128, W_BYTES = 128 * 128, SF_BYTES = 2 * 512;
     static constexpr int STAGE_BYTES = W_BYTES + A_BYTES + 2 * SF_BYTES;
     static constexpr int STAGES = 208 * 1024 / STAGE_BYTES;
     static constexpr int BAR_BYTES = 384;
-    static constexpr int TURN = 33, TURN_BYTES = 4 * 16 * TURN * 4;   // per epilogue warp: 16 rows x 32 columns, padded
+    static constexpr int EPI_WARPS = NT >= 32 ? 8 : 4;
+    static constexpr int TURN = 33, TURN_BYTES = EPI_WARPS * 16 * TURN * 4;   // per epilogue warp: 16 rows x 32 columns, padded
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + BAR_BYTES + TURN_BYTES + 1024;
     static constexpr int SF_COL0 = 2 * NT, SF_COLS = 16;          // per stage: 8 columns for the weights, 8 for A
     static constexpr int PART = 132;                              // row pitch of the partial sums, floats
-    static constexpr int THREADS = 224;
+    static constexpr int THREADS = 32 * (3 + EPI_WARPS);
     static_assert(SF_COL0 + STAGES * SF_COLS <= 512, "TMEM budget");
     static_assert((3 * STAGES + 4) * 8 + 16 <= BAR_BYTES, "barriers");
     static_assert(NT * PART * 4 <= STAGES * STAGE_BYTES, "partial sums");
@@ -183,57 +186,40 @@ __device__ __forceinline__ void skinny_store(const SkinnyParams& p, int m, int n
     else static_cast<float*>(p.d)[n * p.ldd + m] = v;
 }
 
-// One warp stores rows m0.. (16 of them, `rows` exist) x columns n0.. (32) of D; lane = column in r, turned around in `t`.
+// One warp stores rows m0.. (16 of them, `rows` exist) x columns n0.. (32) of D; lane = column in r.  Row-major a lane
+// stores its own column, row by row: the lanes' elements lie together, at any pitch (turned around in shared memory to 16
+// bytes per lane 8.4 against 7.9 us at 512 x 2816, K = 2112, and 10.7 against 9.5 at 128 x 65536, K = 256).  Column-major
+// the rows are turned around in `t`.
 template <int OUT>
 __device__ __forceinline__ void skinny_store16(const SkinnyParams& p, int m0, int rows, int n0, const uint32_t (&r)[16],
                                                float* t) {
-    constexpr int P = SkinnyCfg<16>::TURN;
     const int lane = threadIdx.x & 31;
+    if constexpr (OUT != NVFP4B_OUT_F32_COLMAJOR) {
+        using T = std::conditional_t<OUT == NVFP4B_OUT_BF16_ROWMAJOR, __nv_bfloat16, float>;
+        T* d = static_cast<T*>(p.d) + m0 * p.ldd + n0 + lane;
+        const int mine = n0 + lane < p.N ? rows : 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t[i * P + lane] = p.alpha * __uint_as_float(r[i]);
-    __syncwarp();
-    if constexpr (OUT == NVFP4B_OUT_F32_COLMAJOR) {               // a lane stores four rows of one column
-        const bool whole = p.wide && rows >= 16;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = i * 8 + (lane >> 2), m = 4 * (lane & 3);
-            float* d = static_cast<float*>(p.d) + (long long)(n0 + n) * p.ldd + m0 + m;
-            if (n0 + n >= p.N) continue;
-            if (whole) *reinterpret_cast<float4*>(d) = make_float4(t[m * P + n], t[(m + 1) * P + n], t[(m + 2) * P + n], t[(m + 3) * P + n]);
-            else
-                for (int e = 0; e < 4; ++e)
-                    if (m + e < rows) d[e] = t[(m + e) * P + n];
-        }
+        for (int i = 0; i < 16; ++i, d += p.ldd)
+            if (i < mine) *d = T(p.alpha * __uint_as_float(r[i]));
     } else {
-        if (!p.wide || n0 + 32 > p.N) {                           // a lane stores its own column, row by row
-            if (n0 + lane < p.N)
-                for (int i = 0; i < min(rows, 16); ++i) {
-                    const long long at = (long long)(m0 + i) * p.ldd + n0 + lane;
-                    if constexpr (OUT == NVFP4B_OUT_BF16_ROWMAJOR) static_cast<__nv_bfloat16*>(p.d)[at] = __float2bfloat16_rn(t[i * P + lane]);
-                    else static_cast<float*>(p.d)[at] = t[i * P + lane];
-                }
-            __syncwarp();
-            return;
-        }
-        constexpr int kPer = OUT == NVFP4B_OUT_BF16_ROWMAJOR ? 8 : 4, kLanes = 32 / kPer;   // columns per lane, lanes per row
+        constexpr int P = SkinnyCfg<16>::TURN;
 #pragma unroll
-        for (int i = 0; i < 16 * kLanes / 32; ++i) {
-            const int m = i * (32 / kLanes) + lane / kLanes, n = kPer * (lane % kLanes);
-            const float* v = t + m * P + n;
-            if (m >= rows) continue;
-            if constexpr (OUT == NVFP4B_OUT_BF16_ROWMAJOR) {
-                uint32_t w[4];
+        for (int i = 0; i < 16; ++i) t[i * P + lane] = p.alpha * __uint_as_float(r[i]);
+        __syncwarp();
+        if (p.wide && rows >= 16) {                               // a lane stores four rows of one column
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                    w[e] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.d) + (long long)(m0 + m) * p.ldd + n0 + n) =
-                    make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
-                *reinterpret_cast<float4*>(static_cast<float*>(p.d) + (long long)(m0 + m) * p.ldd + n0 + n) =
-                    make_float4(v[0], v[1], v[2], v[3]);
+            for (int i = 0; i < 4; ++i) {
+                const int n = i * 8 + (lane >> 2), m = 4 * (lane & 3);
+                if (n0 + n < p.N)
+                    *reinterpret_cast<float4*>(static_cast<float*>(p.d) + (n0 + n) * p.ldd + m0 + m) =
+                        make_float4(t[m * P + n], t[(m + 1) * P + n], t[(m + 2) * P + n], t[(m + 3) * P + n]);
             }
+        } else {                                                  // half a warp stores the 16 rows of one column
+            const int m = lane & 15, n1 = m < rows ? min(32, p.N - n0) : 0;
+            float* d = static_cast<float*>(p.d) + (n0 + (lane >> 4)) * p.ldd + m0 + m;
+#pragma unroll
+            for (int n = 0; n < 32; n += 2, d += 2 * p.ldd)
+                if (n + (lane >> 4) < n1) *d = t[m * P + n + (lane >> 4)];
         }
     }
     __syncwarp();
@@ -275,7 +261,7 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 1)
     const int S = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); mbar_init(&sf_full[s], 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 128); }
+        for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 32 * C::EPI_WARPS); }
         *sflag = 0;
         fence_mbar_init();
         prefetch_tmap(&tma_a);
@@ -337,7 +323,7 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 1)
                 if (buf == 0) aphase ^= 1u;
             }
         }
-    } else if (warp == 6) {
+    } else if (warp == 2 + C::EPI_WARPS) {
         if (lane == 0) {
             int stage = 0;
             uint32_t phase = 0;
@@ -361,6 +347,7 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 1)
         }
     } else {
         const int quad = warp & 3, col = quad * 32 + lane;        // column of D within the tile
+        float* my_turn = turn + (warp - 2) * 16 * C::TURN;
         int buf = 0;
         uint32_t aphase = 0;
         for (int t = t0; t < tiles; t += step) {
@@ -370,12 +357,12 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 1)
             tc_fence_after();
             const uint32_t addr = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * NT);
 #pragma unroll 1
-            for (int c0 = 0; c0 < rows; c0 += 16) {
+            for (int c0 = 16 * ((warp - 2) >> 2); c0 < rows; c0 += 4 * C::EPI_WARPS) {
                 uint32_t r[16];
                 tmem_ld_32x32b_x16(addr + c0, r);
                 tmem_wait_ld();
                 if (S == 1) {
-                    skinny_store16<OUT>(p, m0 + c0, rows - c0, nb * 128 + quad * 32, r, turn + quad * 16 * C::TURN);
+                    skinny_store16<OUT>(p, m0 + c0, rows - c0, nb * 128 + quad * 32, r, my_turn);
                 } else {                                          // the stages are free: every load and MMA is done
 #pragma unroll
                     for (int i = 0; i < 16; ++i) reinterpret_cast<uint32_t*>(smem)[(c0 + i) * C::PART + col] = r[i];
@@ -391,15 +378,15 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 1)
     if (S > 1) {                                                  // one tile per cluster
         cluster_sync();
         const int nb = t0 / p.m_tiles, mb = t0 - nb * p.m_tiles;
-        const int rows = min(NT, p.M - mb * NT), e = (warp - 2) & 3;
+        const int rows = min(NT, p.M - mb * NT), e = warp - 2;
         const uint32_t base = smem_u32(smem);
-        if (warp >= 2 && warp < 6) {
+        if (e >= 0 && e < C::EPI_WARPS) {
             // Row-major D: a warp takes a row of the tile, four columns per lane.  Column-major: four columns of the tile,
             // a row per lane.  Either way the lanes' pieces lie together in D, and the padded pitch keeps the 16-byte
             // reads of a quarter-warp on distinct banks.
             constexpr bool COL = OUT == NVFP4B_OUT_F32_COLMAJOR;
             const int items = COL ? 32 * ((rows + 31) / 32) : rows;
-            for (int i = rank * 4 + e; i < items; i += 4 * S) {
+            for (int i = rank * C::EPI_WARPS + e; i < items; i += C::EPI_WARPS * S) {
                 const int c = COL ? (i >> 5) * 32 + lane : i, n = 4 * (COL ? i & 31 : lane);
                 if (COL && c >= rows) continue;
                 const float4 v = cluster_sum(base + 4u * (uint32_t)(c * C::PART + n), S);
