@@ -24,99 +24,41 @@ struct MxGemm {
     long long ldd;
 };
 
-// Epilogue of the CTA-pair tiles.  A thread holds 32 columns of one row; column-major D is stored from there (the lanes'
-// rows lie together), row-major D goes through a shared-memory tile per warp (rows of 16-byte pieces, their order within
-// a row turned by the row number so that neither side meets a bank twice), so that a store instruction writes whole
-// sectors of a few rows: 16 bytes a lane where d's pitch and the tile allow it, else one element a lane (8000 x 11615,
-// K = 320: bf16 114 us, fp32 158 us; 445 and 693 with each lane storing its own row's elements one by one).
-constexpr int kTurnBytes = 32 * 128;                               // per epilogue warp: 32 rows x 32 columns fp32
-using MxPair = PairCfg<5, 8, 8 * kTurnBytes, Kind::MXF4>;
-
-template <bool BF16>
-struct Pieces {
-    static constexpr int kSize = BF16 ? 2 : 4, kPer = 16 / kSize, kLanes = 32 / kPer;   // elements a piece, pieces a row
-
-    // Offset of piece q of row m.
-    static __device__ __forceinline__ int at(int m, int q) {
-        return m * 32 * kSize + ((q ^ (BF16 ? (m >> 1) & 3 : m & 7)) << 4);
-    }
-};
-
-template <int OUT>
+// Epilogue of the CTA-pair tiles, which compute D^T = B A^T: a thread holds 32 columns of one row of the tile, so the lanes'
+// elements lie together in row-major D and each is stored from its register, 64 or 128 bytes of a row per instruction, at
+// any pitch.  The address goes up by additions: with a product for each element 4096 x 7000, K = 512 fp32 took 40.5 us, 27.3
+// so; through a swizzled tile in shared memory to 16 bytes per lane 31.1 (bf16 29.2, 25.9 so).
+template <typename T>
 struct MxEpi {
-    using P = Pieces<OUT == NVFP4B_OUT_BF16_ROWMAJOR>;
-    void* d;
-    long long ldd;
-    int M, N, wide;
+    T* d;
+    long long ldd;                                                 // between the columns of the tile
+    int M, N;                                                      // of D^T
     float alpha;
 
     __device__ __forceinline__ void finish() const {}
 
     template <int CH>
     __device__ __forceinline__ void process(const TileInfo& ti, int row, int col_base, const uint32_t (&r)[CH][32],
-                                            uint8_t* esm) const {
-        const int lane = threadIdx.x & 31, m0 = ti.a_row + row - lane;
-        if (m0 >= M) return;                                       // warp-uniform
-        if constexpr (OUT == NVFP4B_OUT_F32_COLMAJOR) {
-            if (m0 + lane >= M) return;
+                                            uint8_t*) const {
+        const int m = ti.a_row + row;
+        if (m >= M) return;
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const int n0 = ti.n0 + col_base + 32 * c;
-                float* D = static_cast<float*>(d) + m0 + lane;
-                if (n0 >= N) return;
+        for (int c = 0; c < CH; ++c) {
+            const int n0 = ti.n0 + col_base + 32 * c;              // warp-uniform
+            T* at = d + n0 * ldd + m;
+            if (n0 + 32 <= N) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (n0 + i < N) D[(long long)(n0 + i) * ldd] = alpha * __uint_as_float(r[c][i]);
-            }
-        } else {
-            uint8_t* t = esm + ((threadIdx.x >> 5) - 4) * kTurnBytes;   // epilogue warps are 4..
+                for (int i = 0; i < 32; ++i, at += ldd) *at = T(alpha * __uint_as_float(r[c][i]));
+            } else {
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const int n0 = ti.n0 + col_base + 32 * c;          // warp-uniform
-                if (n0 >= N) return;
-#pragma unroll
-                for (int q = 0; q < P::kLanes; ++q) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if constexpr (OUT == NVFP4B_OUT_BF16_ROWMAJOR) {
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(alpha * __uint_as_float(r[c][8 * q + 2 * e]),
-                                                                           alpha * __uint_as_float(r[c][8 * q + 2 * e + 1]));
-                            w[e] = *reinterpret_cast<const uint32_t*>(&h);
-                        } else {
-                            w[e] = __float_as_uint(alpha * __uint_as_float(r[c][4 * q + e]));
-                        }
-                    }
-                    *reinterpret_cast<uint4*>(t + P::at(lane, q)) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-                __syncwarp();
-                store_row_major(t, m0, n0, lane);
-                __syncwarp();
-            }
-        }
-    }
-
-    __device__ __forceinline__ void store_row_major(const uint8_t* t, int m0, int n0, int lane) const {
-        uint8_t* D = static_cast<uint8_t*>(d) + ((long long)m0 * ldd + n0) * P::kSize;
-        if (wide && n0 + 32 <= N) {
-#pragma unroll
-            for (int i = 0; i < P::kLanes; ++i) {
-                const int m = i * P::kPer + lane / P::kLanes, q = lane % P::kLanes;
-                const uint4 v = *reinterpret_cast<const uint4*>(t + P::at(m, q));
-                if (m0 + m < M) *reinterpret_cast<uint4*>(D + (long long)m * ldd * P::kSize + 16 * q) = v;
-            }
-        } else if (n0 + lane < N) {
-            const int rows = min(32, M - m0);
-#pragma unroll 8
-            for (int m = 0; m < rows; ++m) {
-                const uint8_t* v = t + P::at(m, lane / P::kPer) + lane % P::kPer * P::kSize;
-                uint8_t* at = D + ((long long)m * ldd + lane) * P::kSize;
-                if constexpr (OUT == NVFP4B_OUT_BF16_ROWMAJOR) *reinterpret_cast<uint16_t*>(at) = *reinterpret_cast<const uint16_t*>(v);
-                else *reinterpret_cast<uint32_t*>(at) = *reinterpret_cast<const uint32_t*>(v);
+                for (int i = 0; i < 32; ++i, at += ldd)
+                    if (n0 + i < N) *at = T(alpha * __uint_as_float(r[c][i]));
             }
         }
     }
 };
+
+using MxPair = PairCfg<6, 8, 0, Kind::MXF4>;
 
 int mx_core_params(const MxGemm& g, CoreParams& cp) {
     cp.err = device_error_ptr();
@@ -422,7 +364,7 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 1)
 
 // The CTAs that K is split over.  A split saves a CTA k_tiles (1 - 1/S) K-tiles of about 0.27 us and costs the meeting of
 // the partial sums, which grows with the tile's rows and is twice as dear column-major (N = 2816: 16 rows, K = 2816, S = 6
-// 5.2 against 7.3 us unsplit; 128 rows 8.1 and 9.3; K = 704, S = 3 4.9 and 4.6, 8.1 and 6.7), so it is taken from 3 +
+// 5.1 against 7.0 us unsplit; 128 rows 8.0 and 8.3; K = 704, S = 3 4.9 and 4.5, 7.1 and 5.7), so it is taken from 3 +
 // NT / 32 saved K-tiles on, and only as far as all clusters are resident at once (24 clusters of 6 are not: 14.4 us
 // against 8.4 with 4).
 template <int NT>
@@ -498,8 +440,9 @@ int mx_run_skinny(const MxGemm& g, cudaStream_t stream) {
     return err == cudaSuccess ? NVFP4B_OK : record_cuda_error(err);
 }
 
-template <int OUT>
-int mx_run_pair(const MxGemm& g, cudaStream_t stream) {
+template <typename T>
+int mx_run_pair(const MxGemm& g, cudaStream_t stream) {            // g.d as row-major [N, M]
+
     using C = MxPair;
     CUtensorMap ma, mb, msa, msb;
     int st = make_kmajor_map(&ma, g.a, g.M, g.K / 2, C::BM);
@@ -520,20 +463,37 @@ int mx_run_pair(const MxGemm& g, cudaStream_t stream) {
     s.k_tiles = cp.k_tiles;
     const long long tiles = (long long)s.m_tiles * s.n_tiles;
     if (tiles > (1ll << 30)) return NVFP4B_ERR_SHAPE;
-    const int wide = g.ldd % (OUT == NVFP4B_OUT_BF16_ROWMAJOR ? 8 : 4) == 0;          // d is 16-byte aligned
-    return launch_pair<C>(ma, mb, msa, msb, cp, s, MxEpi<OUT>{g.d, g.ldd, g.M, g.N, wide, g.alpha}, (int)tiles, stream);
+    return launch_pair<C>(ma, mb, msa, msb, cp, s, MxEpi<T>{static_cast<T*>(g.d), g.ldd, g.M, g.N, g.alpha}, (int)tiles,
+                          stream);
 }
 
-// The narrow tiles up to 128 rows, and above as long as they make one round (K = 2816: 512 x 4224 9.7 us against 11.1 in
-// CTA-pair tiles, 256 x 8448 10.0 and 11.3; 512 x 8448, two rounds, 14.9 and 12.3).
+// D^T = B A^T, stored where D is: column-major D is row-major D^T.
+MxGemm swapped(const MxGemm& g) { return {g.b, g.b_sf, g.a, g.a_sf, g.alpha, g.N, g.M, g.K, g.d, g.ldd}; }
+
+// Narrow tiles (128 x 128 above 64 rows) or CTA pairs (256 x 256)?  A round of narrow tiles takes about 0.42 us for each
+// K-tile and 0.4 us, 1.3 at least (the stores of one tile under the products of the next); a round of pairs 0.42 us for
+// each K-tile and 1.9 (one accumulator, so the stores are not hidden).  Narrow wins with few K-tiles, with one round, and
+// where the pairs' last round is nearly empty (1024 x 4736, K = 704 7.8 against 10.2 us; 4096 x 7000, K = 512 21.6 and
+// 25.9; K = 1408 37.6 and 34.6; 512 x 8448, K = 2816 13.6 and 11.0).
+bool narrow_tiles(int M, int N, int K) {
+    const long long sms = sm_count(), pairs = sms / 2, kt = (K + 255) / 256;
+    const long long rn = ((M + 127) / 128 * ((N + 127ll) / 128) + sms - 1) / sms;
+    const long long rp = ((M + 255) / 256 * ((N + 255ll) / 256) + pairs - 1) / pairs;
+    return M <= 128 || rn * (kt > 2 ? 2 + 2 * kt : 6) <= rp * (9 + 2 * kt);
+}
+
 template <int OUT>
 int mx_run(const MxGemm& g, cudaStream_t stream) {
+    constexpr bool COL = OUT == NVFP4B_OUT_F32_COLMAJOR;
     if (g.M <= 16) return mx_run_skinny<16, OUT>(g, stream);
     if (g.M <= 32) return mx_run_skinny<32, OUT>(g, stream);
     if (g.M <= 64) return mx_run_skinny<64, OUT>(g, stream);
-    const long long tiles = ((long long)g.N + 127) / 128 * ((g.M + 127) / 128);
-    if (g.M <= 128 || tiles <= sm_count()) return mx_run_skinny<128, OUT>(g, stream);
-    return mx_run_pair<OUT>(g, stream);
+    if constexpr (COL) {                               // from 65 rows on either operand may be the wide one
+        return mx_run<NVFP4B_OUT_F32_ROWMAJOR>(swapped(g), stream);
+    } else {
+        if (narrow_tiles(g.M, g.N, g.K)) return mx_run_skinny<128, OUT>(g, stream);
+        return mx_run_pair<std::conditional_t<OUT == NVFP4B_OUT_BF16_ROWMAJOR, __nv_bfloat16, float>>(swapped(g), stream);
+    }
 }
 
 }  // namespace
