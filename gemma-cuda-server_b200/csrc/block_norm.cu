@@ -6,8 +6,8 @@
 // Persistent CTAs, one row at a time, 8 consecutive elements per thread and chunk.  The rows of y and resid come by
 // bulk copies into a ring of two shared-memory stages, so the next row is on its way while this one goes through its
 // two or three block-wide barriers (a first version with a CTA per row and loads into registers spent its time
-// waiting: 148 us for 8192 x 2816 bf16 with a gate to MXFP4).  NCH chunks per thread: 4 at many rows (small CTAs,
-// several per SM), 1 at few (the shortest path through a row).
+// waiting: 148 us for 8192 x 2816 bf16 with a gate to MXFP4).  NCH chunks per thread: 2 or 4 at many rows (small
+// CTAs, several per SM), 1 at few (the shortest path through a row).
 //
 // The codes stored are those of the float64 z.  With u = 2^-24 a sum of squares is off by at most 17 u of itself (4
 // fused steps and a join per chunk, 3 chunk joins, 5 + 4 tree levels), 1 / rms by 10 u, r by 15 u a with a = |scale|
@@ -33,7 +33,7 @@ __host__ __device__ constexpr int src_size(Src s) { return s == kF32 ? 4 : s == 
 
 constexpr int kNormMaxThreads = 512;
 constexpr int kNormMaxSmem = 220 * 1024;
-constexpr int kRowWarps = 16, kMinRowWarps = 4;          // row kernel: warps per CTA
+constexpr int kRowWarps = 16;                            // row kernel: warps per CTA, at most
 
 struct NormParams {
     nvfp4b_block_norm_args a;
@@ -911,8 +911,11 @@ int raise_smem(const void* kernel, std::atomic<bool> (&ready)[64]) {   // once p
     return NVFP4B_OK;
 }
 
-// The row kernel's launch; `fits` false (nothing launched) where shared memory holds fewer than kMinRowWarps row buffers
-// or a row has more loop steps than a 32-bit mask.
+// The row kernel's launch; `fits` false (nothing launched) where a row has more loop steps than a 32-bit mask, or where the
+// row buffers that shared memory holds are too few.  With y and codes, which is the most to compute, six do (4096 wide,
+// fp32 y and resid, 8192 rows: 122 us, 151 by CTAs; five, 8192 wide bf16: 238 and 243, but 1500 rows 69 and 53).  Else
+// all sixteen, or eight and four rounds of rows (4096 wide, bf16 y and resid to bf16, twelve warps: 8192 rows 55 us, 60 by
+// CTAs; 4096 rows 35 and 32).
 template <Src Y, Src R, bool MX>
 int launch_block_norm_rows(NormParams& p, cudaStream_t s, bool& fits) {
     const auto kernel = block_norm_rows_kernel<Y, R, MX>;
@@ -920,9 +923,10 @@ int launch_block_norm_rows(NormParams& p, cudaStream_t s, bool& fits) {
     p.stage_bytes = (p.a.H * (src_size(Y) + src_size(R)) + 127) / 128 * 128;
     p.weight_bytes = (p.a.H * (Y == kNone ? 2 : 4) + 127) / 128 * 128;
     int warps = (kNormMaxSmem - p.weight_bytes) / p.stage_bytes;
-    fits = warps >= kMinRowWarps && p.a.H <= 32 * 256;
-    if (!fits) return NVFP4B_OK;
     if (warps > kRowWarps) warps = kRowWarps;
+    fits = p.a.H <= 32 * 256 && (MX && Y != kNone ? warps >= 6
+                                                  : warps == kRowWarps || (warps >= 8 && p.a.T / warps >= 4 * sm_count()));
+    if (!fits) return NVFP4B_OK;
     static std::atomic<bool> ready[64];
     const int st = raise_smem(reinterpret_cast<const void*>(kernel), ready);
     if (st) return st;
@@ -952,24 +956,34 @@ int launch_block_norm(NormParams& p, cudaStream_t s) {
     return launch_k(kernel, dim3((unsigned)grid), dim3(threads), smem, s, p);
 }
 
-// From kRowKernelRows rows per SM on a warp per row, where its buffers fit (800 x 2816 fp32 to bf16 9 us, 10 by CTAs; 512
-// rows 7.5 and 6.9).  Below a CTA per row: one chunk per thread, the shortest path through a row, as far as the rows make
-// two rounds (64 x 2816 with y to MXFP4 6.2 us; 512 x 704 3.4 us, 4.7 with four); else four chunks, for more CTAs per SM
-// (512 x 2816 with y to MXFP4 11.8 us, 14.5 with one).
+// From kRowKernelRows rows per SM on a warp per row, where its buffers fit (900 x 2816 with y to MXFP4 16.1 us, 19.6 by
+// CTAs; 700 rows 12.5 that way, 741 by warps 16.2); not with an fp32 y and no codes, where there is little to compute and a
+// row fills much shared memory (2900 x 2816 24.7 us by CTAs, 30.1 by warps).  Below a CTA per row: one chunk per thread,
+// the shortest path through a row, as far as the rows make two rounds (64 x 2816 with y to MXFP4 6.2 us); then two, for more
+// CTAs per SM (512 x 2816 fp32 to bf16 6.1 us, 6.8 with four; 739 x 4096 10.8 and 12.2), or with y and codes, where the
+// threads compute most, four (600 x 2816 12.1 us, 14.8 with two).
 constexpr int kRowKernelRows = 5;
 
-template <Src Y, Src R>
+template <Src Y, Src R, bool MX>
 int dispatch_block_norm(NormParams& p, cudaStream_t s) {   // R = kBf16 without resid
-    if (p.a.T >= kRowKernelRows * sm_count()) {
-        bool fits = false;
-        const int st = p.a.codes ? launch_block_norm_rows<Y, R, true>(p, s, fits)
-                                 : launch_block_norm_rows<Y, R, false>(p, s, fits);
-        if (fits) return st;
+    if constexpr (MX || Y != kF32) {
+        if (p.a.T >= kRowKernelRows * sm_count()) {
+            bool fits = false;
+            const int st = launch_block_norm_rows<Y, R, MX>(p, s, fits);
+            if (fits) return st;
+        }
     }
     const int chunks = p.a.H / 8, resident = kNormMaxThreads / ((chunks + 31) / 32 * 32);    // CTAs per SM, one chunk each
-    const bool wide = resident >= 1 && p.a.T <= 2 * sm_count() * resident;
-    if (p.a.codes) return wide ? launch_block_norm<Y, R, 1, true>(p, s) : launch_block_norm<Y, R, 4, true>(p, s);
-    return wide ? launch_block_norm<Y, R, 1, false>(p, s) : launch_block_norm<Y, R, 4, false>(p, s);
+    if (resident >= 1 && p.a.T <= 2 * sm_count() * resident) return launch_block_norm<Y, R, 1, MX>(p, s);
+    if constexpr (!MX || Y == kNone) {
+        if (chunks <= 2 * kNormMaxThreads) return launch_block_norm<Y, R, 2, MX>(p, s);
+    }
+    return launch_block_norm<Y, R, 4, MX>(p, s);
+}
+
+template <Src Y, Src R>
+int dispatch_block_norm(NormParams& p, cudaStream_t s) {
+    return p.a.codes ? dispatch_block_norm<Y, R, true>(p, s) : dispatch_block_norm<Y, R, false>(p, s);
 }
 
 bool bad_rows(const void* p, int f32, long long ld) { return !aligned16(p) || (ld * (f32 ? 4 : 2)) % 16; }
