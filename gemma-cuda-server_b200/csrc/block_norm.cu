@@ -227,15 +227,15 @@ __device__ __forceinline__ double sum_sq64(const V8& v, bool wild) {
     return ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
 }
 
-// r of a chunk in float64; w = the post weights of the chunk, fgs = scale / rms(y), times the gate unless it is per
-// feature.
+// r of a chunk in float64, by the operations of its definition in their order (an exact zero keeps its sign); w = the post
+// weights of the chunk, fg = 1 / rms(y), times the gate unless it is per feature.
 template <Src Y, Src R>
 __device__ __forceinline__ void r64(const NormParams& p, int row, int ch, const void* sy, const void* sr, const V8& w,
-                                    double fgs, double (&v)[8], bool wild) {
+                                    double fg, double (&v)[8], bool wild) {
     const nvfp4b_block_norm_args& a = p.a;
     const V8 x = a.resid ? load8<R>(sr, ch) : fill8(0.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (double)x.at(i) * (double)a.scale;
+    for (int i = 0; i < 8; ++i) v[i] = (double)x.at(i);
     if constexpr (Y != kNone) {
         const V8 n = load8<Y>(sy, ch);
         const bool g_col = a.gate && a.gate_col_stride;
@@ -243,9 +243,11 @@ __device__ __forceinline__ void r64(const NormParams& p, int row, int ch, const 
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const double t = Y == kBf16 && !wild ? (double)(n.at(i) * w.at(i)) : (double)n.at(i) * (double)w.at(i);
-            v[i] = fma(g_col ? t * (double)g.at(i) : t, fgs, v[i]);
+            v[i] = fma(g_col ? t * (double)g.at(i) : t, fg, v[i]);
         }
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= (double)a.scale;
 }
 
 // Whether a mean of squares (+ eps) is in the range where its fp32 value has its relative error bound.
@@ -420,18 +422,18 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
 
         const bool again = MX ? __syncthreads_or(wild || redo != 0) != 0 : wild;
         if (again) {                                     // sums of the row in float64; inputs from the stage again
-            double fgs64 = (double)a.scale * (double)g_row.x;
+            double fg64 = (double)g_row.x;
             if (HAS_Y && a.post_norm) {
                 double s = 0.0;
 #pragma unroll 1
                 for (int ch = tid; ch < chunks; ch += threads) s += sum_sq64<Y>(load8<Y == kF32 ? kF32 : kBf16>(sy, ch), wild);
-                fgs64 *= rsqrt(block_sum(s, red64[0]) / a.H + (double)a.eps);
+                fg64 *= rsqrt(block_sum(s, red64[0]) / a.H + (double)a.eps);
             }
             double s = 0.0;
 #pragma unroll 1
             for (int ch = tid; ch < chunks; ch += threads) {
                 double v[8];
-                r64<Y, R>(p, row, ch, sy, sr, HAS_Y ? weight8(a.post_weight, ch) : V8(), fgs64, v, wild);
+                r64<Y, R>(p, row, ch, sy, sr, HAS_Y ? weight8(a.post_weight, ch) : V8(), fg64, v, wild);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) s = fma(v[i], v[i], s);
             }
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = 0.0;
                 if (need && ch < chunks) {
-                    r64<Y, R>(p, row, ch, sy, sr, HAS_Y ? weight8(a.post_weight, ch) : V8(), fgs64, v, wild);
+                    r64<Y, R>(p, row, ch, sy, sr, HAS_Y ? weight8(a.post_weight, ch) : V8(), fg64, v, wild);
                     const V8 w = weight8(a.norm_weight, ch);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -525,26 +527,28 @@ struct Row64 {
     const uint4* w_post;
     int row, chunks;
     bool has_v, g_col, wild;
-    double fgs, f, scale;
+    double fg, f, scale;
 
     __device__ __forceinline__ void r8(int ch, double (&r)[8]) const {
         const V8 x = load8<R>(v, ch);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) r[k] = has_v ? scale * (double)x.at(k) : 0.0;
+        for (int k = 0; k < 8; ++k) r[k] = has_v ? (double)x.at(k) : 0.0;
         if constexpr (Y != kNone) {
             const V8 n = load8<Y>(y, ch), w = unpack8(w_post[ch]);
             if (g_col) {
                 const V8 g = gate8(p, row, ch);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) r[k] = fma((double)n.at(k) * (double)w.at(k) * (double)g.at(k), fgs, r[k]);
+                for (int k = 0; k < 8; ++k) r[k] = fma((double)n.at(k) * (double)w.at(k) * (double)g.at(k), fg, r[k]);
             } else if (Y == kBf16 && !wild) {                       // an exact fp32 product: one conversion for two
 #pragma unroll
-                for (int k = 0; k < 8; ++k) r[k] = fma((double)(n.at(k) * w.at(k)), fgs, r[k]);
+                for (int k = 0; k < 8; ++k) r[k] = fma((double)(n.at(k) * w.at(k)), fg, r[k]);
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) r[k] = fma((double)n.at(k) * (double)w.at(k), fgs, r[k]);
+                for (int k = 0; k < 8; ++k) r[k] = fma((double)n.at(k) * (double)w.at(k), fg, r[k]);
             }
         }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) r[k] *= scale;
     }
     // Sum over the row of the squares of y, or of r.
     template <bool OF_Y>
@@ -571,8 +575,8 @@ struct Row64 {
           wild(wild_), scale((double)p_.a.scale) {
         const double h = (double)p.a.H, eps = (double)p.a.eps;
         g_col = Y != kNone && p.a.gate && p.a.gate_col_stride;
-        fgs = scale * (Y != kNone && p.a.gate && !g_col ? (double)gate_at(p.a, row, 0) : 1.0);
-        if (Y != kNone && p.a.post_norm) fgs *= rsqrt(sum_sq<true>() / h + eps);
+        fg = Y != kNone && p.a.gate && !g_col ? (double)gate_at(p.a, row, 0) : 1.0;
+        if (Y != kNone && p.a.post_norm) fg *= rsqrt(sum_sq<true>() / h + eps);
         f = rsqrt(sum_sq<false>() / h + eps);
     }
 };
@@ -846,7 +850,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
                     const bool unsure = code != other || ((top ^ bot) & 0x7F800000u) != 0u ||
                                         top - 0x08800000u >= 0x7F000000u - 0x08800000u;
                     doubt |= unsure && top != 0u ? 1u << i : 0u;
-                    if (ok) code_row[ch] = code;
+                    // zeros that agree: the end that kept their sign (x - 0 of each, or x + x rel)
+                    if (ok) code_row[ch] = HAS_Y ? code : other;
                     uint32_t w = ok ? ((field >> 23) - 2u) << (8 * ((lane & 15) >> 2)) : 0u;
                     w |= __shfl_xor_sync(0xFFFFFFFFu, w, 4);
                     w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
@@ -913,7 +918,8 @@ int raise_smem(const void* kernel, std::atomic<bool> (&ready)[64]) {   // once p
 
 // The row kernel's launch; `fits` false (nothing launched) where a row has more loop steps than a 32-bit mask, or where the
 // row buffers that shared memory holds are too few.  With y and codes, which is the most to compute, six do (4096 wide,
-// fp32 y and resid, 8192 rows: 122 us, 151 by CTAs; five, 8192 wide bf16: 238 and 243, but 1500 rows 69 and 53).  Else
+// fp32 y and resid, 8192 rows: 122 us, 151 by CTAs; five, 8192 wide bf16: 238 and 243, but 1500 rows 69 and 53), if the
+// scale is positive: it goes into the sum's terms there, which a scale below or at zero would give zeros of another sign.  Else
 // all sixteen, or eight and four rounds of rows (4096 wide, bf16 y and resid to bf16, twelve warps: 8192 rows 55 us, 60 by
 // CTAs; 4096 rows 35 and 32).
 template <Src Y, Src R, bool MX>
@@ -924,7 +930,7 @@ int launch_block_norm_rows(NormParams& p, cudaStream_t s, bool& fits) {
     p.weight_bytes = (p.a.H * (Y == kNone ? 2 : 4) + 127) / 128 * 128;
     int warps = (kNormMaxSmem - p.weight_bytes) / p.stage_bytes;
     if (warps > kRowWarps) warps = kRowWarps;
-    fits = p.a.H <= 32 * 256 && (MX && Y != kNone ? warps >= 6
+    fits = p.a.H <= 32 * 256 && (MX && Y != kNone ? warps >= 6 && p.a.scale > 0.f
                                                   : warps == kRowWarps || (warps >= 8 && p.a.T / warps >= 4 * sm_count()));
     if (!fits) return NVFP4B_OK;
     static std::atomic<bool> ready[64];

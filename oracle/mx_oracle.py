@@ -74,17 +74,16 @@ def rms(x: np.ndarray, eps: float) -> np.ndarray:
 
 
 def block_norm(resid=None, norm_weight=None, eps=1e-6, y=None, post_weight=None, post_norm=None, gate=None, scale=1.0):
-    """(r, z): r = scale (resid + gate * [rms](y) post_weight), z = rms(r) norm_weight; all float64."""
-    r = np.zeros(1)
+    """(r, z): r = scale (resid + gate * [rms](y) post_weight), z = rms(r) norm_weight; all float64.  Without y r = scale
+    resid; a resid of None is 0, so a zero that y alone gives is +0 before the scale."""
+    r = resid
     if y is not None:
         n = np.asarray(y, np.float64)
         if post_norm if post_norm is not None else post_weight is not None:
             n = rms(n, eps)
         if post_weight is not None:
             n = n * post_weight
-        r = n if gate is None else n * gate
-    if resid is not None:
-        r = r + resid
-    r = r * scale
+        r = (n if gate is None else n * gate) + (0.0 if resid is None else resid)
+    r = np.asarray(r, np.float64) * scale
     z = rms(r, eps)
     return r, z if norm_weight is None else z * norm_weight

@@ -163,6 +163,31 @@ def test_rows_that_cancel_vanish_or_overflow(T, dtype):
     assert np.array_equal(_n(out)[~whole], z[~whole], equal_nan=True)
 
 
+@pytest.mark.parametrize("T", [6, 1300])
+@pytest.mark.parametrize("scale", [1.0, 0.7, -1.3, 0.0, -0.0])
+@pytest.mark.parametrize("resid,y", [(B, None), (F, None), (B, B), (F, F), (None, B)])
+def test_signs_of_zeros(T, scale, resid, y):
+    """Codes keep the sign of a zero: resid + y that cancels exactly, zeros of either sign, a scale that is not positive."""
+    p = require_gpu()
+    kw = _make(T, 160, 30, resid, y, post=False)
+    for k in ("resid", "y"):
+        if kw.get(k) is not None:
+            kw[k][0], kw[k][1], kw[k][2, 3], kw[k][3, :40] = 0.0, -0.0, -0.0, -0.0
+            kw[k][4, ::3] = -0.0 if k == "y" else 0.0
+            kw[k][5, 32:96] = 0.0 if k == "y" else -0.0
+    if resid and y:
+        kw["y"][2, 8:48] = -kw["resid"][2, 8:48]
+        kw["resid"][3, 64] = 2.0 ** -3
+        kw["y"][3, 64] = -(2.0 ** -3)
+    codes, scales = poisoned(T * 80).view(T, 80), poisoned(mx.scale_buffer_bytes(T, 160))
+    p.block_norm(codes=codes, scales=scales, scale=scale, **kw)
+    ref = mx.quantize(_want({**kw, "scale": scale})[1])
+    byte, _ = mx.untile_scales(scales.cpu().numpy(), T, 160)
+    assert np.array_equal(byte, ref[1])
+    bad = np.argwhere(codes.cpu().numpy() != ref[0])
+    assert len(bad) == 0, bad[:6].tolist()
+
+
 @pytest.mark.parametrize("T", [12, 1300])
 def test_weights_that_are_not_finite(T):
     """A NaN or infinite weight of the second norm spoils exactly its block of every row."""
