@@ -171,7 +171,8 @@ __device__ __noinline__ bool geglu_tiny(const uint16_t* gp, const uint16_t* up, 
 // g * rcp(1 + ex2(-w)) * u is off by at most |h| e, e = max(-w, 1) 2^-22 + 2^-20: the roundings of w leave it 3.5 * 2^-24
 // off, so the exponential 2.5 |w| 2^-24, which for w > 0 enters through ex2(-w) / (1 + ex2(-w)) only (below 1 / w);
 // ex2.approx 2^-22, the sum, the reciprocal and the products add 9 * 2^-24, h - d and h + d the rest.  The .ftz forms flush
-// where w > 126 (the exponential adds nothing to 1) or w < -100 (no bound there, below).
+// where w > 126 (the exponential adds nothing to 1) or w < -100 (no bound there, below).  From g = -1.5e13 down w is an
+// infinity, and so is e: 0 * e makes both ends NaN, whose codes agree, so those blocks are redone by the size of w.
 template <bool WIDE>
 __global__ void __launch_bounds__(kMxThreads) mx_geglu_kernel(const uint16_t* __restrict__ x, long long ldx, int M,
                                                               int I, uint8_t* __restrict__ codes,
@@ -216,7 +217,8 @@ __global__ void __launch_bounds__(kMxThreads) mx_geglu_kernel(const uint16_t* __
         const float inv = __uint_as_float(0x80000000u - field);
         const float total = sum.x + sum.y;                             // NaN where an h is (no maximum shows it)
         bool redo = ((hi ^ lo) & 0x7F800000u) != 0u || hi >= 0x7F000000u || !(total == total);
-        if (p.ok && (w_min <= -100.f || hi < 0x12800000u)) redo |= geglu_tiny(gp, gp + I, top);   // 2^-90
+        if (p.ok && (w_min <= -100.f || hi < 0x12800000u))                                    // 2^-90
+            redo |= w_min < -0x1p127f || geglu_tiny(gp, gp + I, top);
         uint32_t c[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {

@@ -150,3 +150,38 @@ def test_graph_replay_and_side_stream():
         want = mx.quantize(x.double().cpu().numpy())
         _check(codes, scales, want, 96, 704)
         assert np.array_equal(v.double().cpu().numpy(), mx.dequantize(*want))
+
+
+@pytest.mark.parametrize("gate", [-3e12, -1.5e13, -2e13, -1e19, -1e20, -1e38, -3.3895313892515355e38, 1e19, 1e38])
+def test_geglu_gates_beyond_the_fp32_cube(gate):
+    """Gates whose cube leaves fp32, among ordinary ones: h is a signed zero (or g u), whatever the up value beside it."""
+    p = require_gpu()
+    rng = np.random.default_rng(1)
+    rows = []
+    for u in (1.0, -1.0, 0.0, -0.0, 1e-20, -1e30, 3e38):
+        for at in ([3], [0, 31], list(range(16)), list(range(16, 32)), list(range(0, 32, 2))):
+            for g0, u0 in ((np.ones(32), np.arange(32.0)), (rng.normal(0, 1.5, 32), rng.normal(0, 1, 32)),
+                           (np.full(32, -9.0), np.ones(32)), (np.full(32, 1e-30), np.ones(32)), (np.zeros(32), np.ones(32))):
+                g1, u1 = g0.copy(), u0.copy()
+                g1[at], u1[at] = gate, u
+                rows.append((g1, u1))
+    n = len(rows)                                              # one block each, all of them in the rows of one call
+    g, u = (torch.tensor(np.array([r[i] for r in rows])).to(torch.bfloat16) for i in range(2))
+    want = mx.quantize(mx.geglu(g.double().numpy(), u.double().numpy()))
+    _check(*_run(p.mx_geglu_quantize, torch.cat([g, u], 1).cuda(), n, 32), want, n, 32)
+    wide = [t.view(5, -1) for t in (g, u)]                     # and side by side: the other threads of the warp
+    k = wide[0].shape[1]
+    want = mx.quantize(mx.geglu(wide[0].double().numpy(), wide[1].double().numpy()))
+    _check(*_run(p.mx_geglu_quantize, torch.cat(wide, 1).cuda(), 5, k), want, 5, k)
+
+
+def test_geglu_masked_gates():
+    """A padded batch: gates of the type's lowest value wherever a token or a feature is masked."""
+    p = require_gpu()
+    g = torch.Generator().manual_seed(4)
+    gate, up = (torch.randn(150, 704, generator=g).bfloat16() for _ in range(2))
+    gate[100:] = torch.finfo(torch.bfloat16).min
+    gate[:, 650:] = torch.finfo(torch.bfloat16).min
+    gate[::7, ::5] = torch.finfo(torch.bfloat16).min
+    want = mx.quantize(mx.geglu(gate.double().numpy(), up.double().numpy()))
+    _check(*_run(p.mx_geglu_quantize, torch.cat([gate, up], 1).cuda(), 150, 704), want, 150, 704)
