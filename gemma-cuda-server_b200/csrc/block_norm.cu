@@ -16,6 +16,11 @@
 // without y (r is one product) by 16 u |z|.  Where the codes of z - d and z + d differ (one row in eight at 2816
 // elements; one in forty without y), or a sum of squares leaves the range in which the bounds hold, the CTA takes the
 // row's sums in float64 and redoes the blocks that need it.
+//
+// Products are taken as (x f) w, f = 1 / rms(x): |x f| is at most sqrt(H), so what overflows is an overflow of the result,
+// while w f may leave fp32 at either end for finite values (w = 2^121 over rows of 2^-14 gave NaN for their zeros).  What
+// underflows is off by 2^-150 times the factors behind it; a block is redone where its maximum is below 2^-60, beside
+// which that does not count as long as 1 / rms(r) and the two weights of an element make less than 2^60.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -326,6 +331,8 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                 if (ch >= chunks) continue;
                 const V8 w = weight8(a.post_weight, ch);
                 const V8 v = a.resid ? load8<R>(sr, ch) : fill8(0.f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[c].p[j] = __fmul2_rn(__fmul2_rn(r[c].p[j], fg), w.p[j]);
                 if (a.gate && a.gate_col_stride) {
                     const V8 g = gate8(p, row, ch);
 #pragma unroll
@@ -334,7 +341,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                 float2 s2 = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 t = __fmul2_rn(r[c].p[j], __fmul2_rn(w.p[j], fg));
+                    const float2 t = r[c].p[j];
                     r[c].p[j] = __fmul2_rn(__fadd2_rn(v.p[j], t), scale);
                     if constexpr (MX) {
                         const float2 b = make_float2(fabsf(v.p[j].x) + fabsf(t.x), fabsf(v.p[j].y) + fabsf(t.y));
@@ -383,7 +390,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                 float2 all = make_float2(0.f, 0.f);      // NaN if a z is (a NaN weight passes every maximum)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    z[c].p[j] = __fmul2_rn(r[c].p[j], __fmul2_rn(w.p[j], f2));
+                    z[c].p[j] = __fmul2_rn(__fmul2_rn(r[c].p[j], f2), w.p[j]);
                     if constexpr (MX) all = __fadd2_rn(all, z[c].p[j]);
                     zm = fmaxf(zm, fmaxf(fabsf(z[c].p[j].x), fabsf(z[c].p[j].y)));
                     if (MX && HAS_Y) wm = fmaxf(wm, fmaxf(fabsf(w.p[j].x), fabsf(w.p[j].y)));
@@ -412,7 +419,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                     const uint32_t up = cvt_e2m1x8(hi[0].x, hi[0].y, hi[1].x, hi[1].y, hi[2].x, hi[2].y, hi[3].x, hi[3].y);
                     const bool doubt = code[c] != up || byte[c] != mx_byte(__float_as_uint(fmaxf(zm - dm, 0.f))) ||
                                        top_bits >= 0x7F000000u ||
-                                       (top_bits != 0u && top_bits < 0x08800000u) ||  // below 2^-110 no relative bounds
+                                       (top_bits != 0u && top_bits < 0x21800000u) ||  // below 2^-60
                                        !(all.x + all.y == all.x + all.y);
                     redo |= doubt ? 1u << c : 0u;
                 }
@@ -737,7 +744,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
                 const V8 y = load8<Y>(sy, ch), w = unpack8(w_post[ch]), v = a.resid ? load8<R>(sr, ch) : fill8(0.f);
                 V8 t, r;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) t.p[j] = __fmul2_rn(y.p[j], __fmul2_rn(w.p[j], fgs2));
+                for (int j = 0; j < 4; ++j) t.p[j] = __fmul2_rn(__fmul2_rn(y.p[j], fgs2), w.p[j]);
                 if (g_col) {
                     const V8 g = gate8(p, row, ch);
 #pragma unroll
@@ -794,7 +801,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
             const V8 w = unpack8(w_norm[ch]);
             V8 z;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) z.p[j] = __fmul2_rn(r.p[j], __fmul2_rn(w.p[j], f2));
+            for (int j = 0; j < 4; ++j) z.p[j] = __fmul2_rn(__fmul2_rn(r.p[j], f2), w.p[j]);
             return z;
         };
         uint32_t row_max = 0, doubt = 0;                            // bit i: the chunk of loop step i is not proven
@@ -848,7 +855,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
                         cvt_e2m1x8(hi[0].x, hi[0].y, hi[1].x, hi[1].y, hi[2].x, hi[2].y, hi[3].x, hi[3].y);
                     // also where the exponent is in doubt, or the values are near the ends of the range
                     const bool unsure = code != other || ((top ^ bot) & 0x7F800000u) != 0u ||
-                                        top - 0x08800000u >= 0x7F000000u - 0x08800000u;
+                                        top - 0x21800000u >= 0x7F000000u - 0x21800000u;
                     doubt |= unsure && top != 0u ? 1u << i : 0u;
                     // zeros that agree: the end that kept their sign (x - 0 of each, or x + x rel)
                     if (ok) code_row[ch] = HAS_Y ? code : other;

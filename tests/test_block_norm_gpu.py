@@ -341,3 +341,54 @@ def test_refusals():
         p.block_norm(torch.zeros(4, 66, device="cuda")[:, :64], w)
     with pytest.raises(p.NvFp4Error, match="ARG"):
         p.block_norm(x, w, eps=-1.0)
+
+
+@pytest.mark.parametrize("T", [12, 1300])
+@pytest.mark.parametrize("resid,y", [(B, None), (F, None), (B, B), (F, F), (None, B)])
+def test_weight_times_reciprocal_rms_beyond_fp32(T, resid, y):
+    """Small rows under large weights: w / rms leaves fp32, w (x / rms) does not -- codes, out and resid_out."""
+    p = require_gpu()
+    H = 160
+    kw = _make(T, H, 21, resid, y)
+    for k in ("resid", "y"):
+        if kw.get(k) is not None:
+            kw[k] *= 2.0 ** -14
+            kw[k][:, 5:40:3], kw[k][2], kw[k][:, 64:96] = 0.0, 0.0, 0.0
+    kw["norm_weight"][::2] = 2.0 ** 121                       # 1 / rms is up to 2^10 (eps), z below 2^127
+    _check(p, T, H, True, True, **kw)
+    _check(p, T, H, True, False, **kw)
+    _check(p, T, H, False, True, **kw)
+    if y:
+        kw["post_weight"] = kw["norm_weight"]
+        kw["norm_weight"] = None
+        r, _, dr, _ = _want(kw)
+        out = torch.empty(T, H, dtype=F, device="cuda")
+        p.block_norm(**kw, resid_out=out)
+        _near(out, r, dr, F)
+        _check(p, T, H, True, True, **kw)
+
+
+@pytest.mark.parametrize("T", [12, 1300])
+def test_products_that_underflow(T):
+    """Blocks whose second weights, gates or inputs lie many powers of two below the row's."""
+    p = require_gpu()
+    H = 256
+    for resid, y, gate in [(F, None, ""), (B, None, ""), (F, F, "feature"), (B, B, "row"), (None, F, "feature")]:
+        kw = _make(T, H, 23, resid, y, gate=gate)
+        kw["norm_weight"][32:64] *= 2.0 ** -70
+        kw["norm_weight"][64:96] *= 2.0 ** -120
+        for k in ("resid", "y"):
+            if kw.get(k) is not None:
+                kw[k][:, 96:128] *= 2.0 ** -80
+                kw[k][:, 128:160] *= 2.0 ** -126
+                kw[k][3] *= 2.0 ** 45
+                kw[k][5] *= 2.0 ** 60
+        if gate == "feature":
+            kw["gate"][160:192] *= 2.0 ** -100
+            kw["gate"][192:224] *= 2.0 ** -140
+        if gate == "row":
+            kw["gate"][6], kw["gate"][7] = 2.0 ** -100, 2.0 ** -130
+        if y:
+            kw["post_weight"][224:240] *= 2.0 ** -110
+        _check(p, T, H, True, False, **kw)
+        _check(p, T, H, True, False, eps=0.0, **kw)
