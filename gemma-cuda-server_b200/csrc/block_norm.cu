@@ -373,7 +373,10 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                 const float2 s = block_sum2(make_float2(ss, sa), red_r[odd]);
                 ss = s.x;
                 const float k = fabsf(a.scale) * sqrtf(s.y / ss);
-                rel = s.y > 0.f ? fmaf(k, 0x1p-20f, 0x1.cp-20f) : 0.f;
+                if (s.y < 0x1p-100f)                     // lost bits; unless scale brings r back, m is eps (or out of
+                    rel = fabsf(a.scale) <= 32.f ? 0x1.cp-20f : 1.f;   // range) and k does not enter
+                else
+                    rel = fmaf(k, 0x1p-20f, 0x1.cp-20f);
                 wild |= !(rel < 0x1p-12f);               // also where ss = 0 < sa: r cancelled altogether
             } else {
                 ss = block_sum(ss, reinterpret_cast<float*>(red_r[odd]));

@@ -368,6 +368,31 @@ def test_weight_times_reciprocal_rms_beyond_fp32(T, resid, y):
         _check(p, T, H, True, True, **kw)
 
 
+def _borders(shape, size, seed):
+    """fp32 values within three steps of the rounding borders of an MXFP4 block whose largest is 4.5 (each block has one),
+    times `size`, a power of two; either sign."""
+    rng = np.random.default_rng(seed)
+    x = rng.choice(np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], np.float32), shape)
+    x = (x.view(np.int32) + rng.integers(-3, 4, shape, dtype=np.int32)).view(np.float32)
+    x.reshape(-1, 32)[:, 9] = 4.5
+    return torch.from_numpy(x * rng.choice(np.array([-1, 1], np.float32), shape) * np.float32(size)).cuda()
+
+
+@pytest.mark.parametrize("T", [12, 739, 800])
+@pytest.mark.parametrize("eps", [2.0 ** -20, 2.0 ** -60])
+@pytest.mark.parametrize("e", [-60, -70, -74, -78, -85, -100, -110, -125])
+def test_rows_whose_squares_underflow(T, eps, e):
+    """Rows so far below eps that the norms only multiply by 1 / sqrt(eps), near the rounding borders of their codes."""
+    p = require_gpu()
+    H = 160
+    r, one = _borders((T, H), 2.0 ** e, T - e), torch.ones(H, dtype=B, device="cuda")
+    for scale in (1.0, 0.7, 2.0 ** 30):
+        x = r * (1 / scale)                                   # 0.7: near the borders, seldom on one
+        for kw in (dict(resid=x), dict(y=x), dict(y=x, post_weight=one), dict(resid=x, y=x), dict(resid=0.25 * x, y=0.5 * x),
+                   dict(resid=-x, y=2.0 * x), dict(resid=x, y=x, gate=torch.full((T, 1), 0.5, device="cuda"))):
+            _check(p, T, H, True, False, eps=eps, scale=scale, **kw)
+
+
 @pytest.mark.parametrize("T", [12, 1300])
 def test_products_that_underflow(T):
     """Blocks whose second weights, gates or inputs lie many powers of two below the row's."""
