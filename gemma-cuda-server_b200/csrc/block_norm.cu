@@ -220,9 +220,32 @@ __device__ __forceinline__ void zero_padding_rows(const NormParams& p) {
                                                                 p.tile_cols)) = 0u;
 }
 
-// The float64 redo of a row: the products of two bf16 values are exact in fp32 (but for overflow and underflow, which
-// only a `wild` row may hold), so those of bf16 sources are converted after the product: the conversions, at an eighth
-// of the fp32 rate, are what the redo costs.
+// The float64 redo of a row: conversions, at an eighth of the fp32 rate, are what it costs.  The product of two bf16 values
+// is exact in fp32, but for underflow and overflow, and then one conversion serves both.  Squares: only a `wild` row holds
+// any whose underflow or overflow counts in the sum.  y post_weight: such a product may be all that an element is made of,
+// so chunks with one that is 0 or below 2^-130 (16 bits end at 2^-149 from 2^-134 down), or infinite, go the long way.
+template <Src Y>
+__device__ __forceinline__ void weighted64(const V8& y, const V8& w, double (&t)[8]) {
+    bool exact = Y == kBf16;
+    if constexpr (Y == kBf16) {
+        float lo = __int_as_float(0x7F800000), hi = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float q = fabsf(y.at(i) * w.at(i));
+            lo = fminf(lo, q);
+            hi = fmaxf(hi, q);
+        }
+        exact = lo > 0x1p-130f && hi < __int_as_float(0x7F800000);
+    }
+    if (exact) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = (double)(y.at(i) * w.at(i));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = (double)y.at(i) * (double)w.at(i);
+    }
+}
+
 template <Src S>
 __device__ __forceinline__ double sum_sq64(const V8& v, bool wild) {
     double q[8];
@@ -236,20 +259,18 @@ __device__ __forceinline__ double sum_sq64(const V8& v, bool wild) {
 // weights of the chunk, fg = 1 / rms(y), times the gate unless it is per feature.
 template <Src Y, Src R>
 __device__ __forceinline__ void r64(const NormParams& p, int row, int ch, const void* sy, const void* sr, const V8& w,
-                                    double fg, double (&v)[8], bool wild) {
+                                    double fg, double (&v)[8]) {
     const nvfp4b_block_norm_args& a = p.a;
     const V8 x = a.resid ? load8<R>(sr, ch) : fill8(0.f);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (double)x.at(i);
     if constexpr (Y != kNone) {
-        const V8 n = load8<Y>(sy, ch);
         const bool g_col = a.gate && a.gate_col_stride;
         const V8 g = g_col ? gate8(p, row, ch) : fill8(1.f);
+        double t[8];
+        weighted64<Y>(load8<Y>(sy, ch), w, t);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const double t = Y == kBf16 && !wild ? (double)(n.at(i) * w.at(i)) : (double)n.at(i) * (double)w.at(i);
-            v[i] = fma(g_col ? t * (double)g.at(i) : t, fg, v[i]);
-        }
+        for (int i = 0; i < 8; ++i) v[i] = fma(g_col ? t[i] * (double)g.at(i) : t[i], fg, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= (double)a.scale;
@@ -443,7 +464,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
 #pragma unroll 1
             for (int ch = tid; ch < chunks; ch += threads) {
                 double v[8];
-                r64<Y, R>(p, row, ch, sy, sr, HAS_Y ? weight8(a.post_weight, ch) : V8(), fg64, v, wild);
+                r64<Y, R>(p, row, ch, sy, sr, HAS_Y ? weight8(a.post_weight, ch) : V8(), fg64, v);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) s = fma(v[i], v[i], s);
             }
@@ -462,7 +483,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = 0.0;
                 if (need && ch < chunks) {
-                    r64<Y, R>(p, row, ch, sy, sr, HAS_Y ? weight8(a.post_weight, ch) : V8(), fg64, v, wild);
+                    r64<Y, R>(p, row, ch, sy, sr, HAS_Y ? weight8(a.post_weight, ch) : V8(), fg64, v);
                     const V8 w = weight8(a.norm_weight, ch);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
@@ -528,7 +549,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
 }
 
 // A row in float64 by a warp.  y and v: the rows of y and resid (valid memory without resid too), in global or shared
-// memory.  A chunk's 24 values are loaded before any is used and no branch parts them: written element by element, each
+// memory.  A chunk's 24 values are loaded before any is used, by no branch apart: written element by element, each
 // behind its bounds check, a row of 2816 took 32,000 cycles of exposed latencies instead of about 5,000.
 template <Src Y, Src R>
 struct Row64 {
@@ -536,7 +557,7 @@ struct Row64 {
     const void *y, *v;
     const uint4* w_post;
     int row, chunks;
-    bool has_v, g_col, wild;
+    bool has_v, g_col;
     double fg, f, scale;
 
     __device__ __forceinline__ void r8(int ch, double (&r)[8]) const {
@@ -545,16 +566,15 @@ struct Row64 {
         for (int k = 0; k < 8; ++k) r[k] = has_v ? (double)x.at(k) : 0.0;
         if constexpr (Y != kNone) {
             const V8 n = load8<Y>(y, ch), w = unpack8(w_post[ch]);
+            double t[8];
+            weighted64<Y>(n, w, t);
             if (g_col) {
                 const V8 g = gate8(p, row, ch);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) r[k] = fma((double)n.at(k) * (double)w.at(k) * (double)g.at(k), fg, r[k]);
-            } else if (Y == kBf16 && !wild) {                       // an exact fp32 product: one conversion for two
-#pragma unroll
-                for (int k = 0; k < 8; ++k) r[k] = fma((double)(n.at(k) * w.at(k)), fg, r[k]);
+                for (int k = 0; k < 8; ++k) r[k] = fma(t[k] * (double)g.at(k), fg, r[k]);
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) r[k] = fma((double)n.at(k) * (double)w.at(k), fg, r[k]);
+                for (int k = 0; k < 8; ++k) r[k] = fma(t[k], fg, r[k]);
             }
         }
 #pragma unroll
@@ -579,10 +599,9 @@ struct Row64 {
         }
         return warp_sum(s);
     }
-    __device__ __forceinline__ Row64(const NormParams& p_, int row_, const void* y_, const void* v_, const uint4* w_post_,
-                                     bool wild_)
+    __device__ __forceinline__ Row64(const NormParams& p_, int row_, const void* y_, const void* v_, const uint4* w_post_)
         : p(p_), y(y_), v(v_), w_post(w_post_), row(row_), chunks(p_.a.H >> 3), has_v(p_.a.resid != nullptr),
-          wild(wild_), scale((double)p_.a.scale) {
+          scale((double)p_.a.scale) {
         const double h = (double)p.a.H, eps = (double)p.a.eps;
         g_col = Y != kNone && p.a.gate && p.a.gate_col_stride;
         fg = Y != kNone && p.a.gate && !g_col ? (double)gate_at(p.a, row, 0) : 1.0;
@@ -598,7 +617,7 @@ __device__ __noinline__ uint32_t redo_row64(const NormParams& p, int row, uint32
                                             const void* v, const uint4* w_post, const uint4* w_norm) {
     const nvfp4b_block_norm_args& a = p.a;
     const int lane = threadIdx.x & 31;
-    const Row64<Y, R> q(p, row, y, v, w_post, wild);
+    const Row64<Y, R> q(p, row, y, v, w_post);
     __syncwarp();                                                   // codes and scale words stored before come first
     uint32_t zmax = 0;
     int step = 0;

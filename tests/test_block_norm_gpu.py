@@ -394,6 +394,23 @@ def test_rows_whose_squares_underflow(T, eps, e):
 
 
 @pytest.mark.parametrize("T", [12, 1300])
+@pytest.mark.parametrize("y_exp,w_exp", [(-30, -108), (-30, -112), (-60, -84), (0, -126), (20, -126)])
+def test_products_of_input_and_weight_that_underflow(T, y_exp, w_exp):
+    """A block whose y post_weight needs bits below the smallest fp32, brought back by the second weights."""
+    p = require_gpu()
+    for resid in (None, B, F):
+        kw = _make(T, 256, 24, resid, B)
+        kw["y"][:, 224:] *= 2.0 ** y_exp
+        kw["post_weight"][224:] *= 2.0 ** w_exp
+        kw["norm_weight"][224:] *= 2.0 ** 45
+        if resid:
+            kw["resid"][:, 224:] = 0
+        _check(p, T, 256, True, False, **kw)
+        _check(p, T, 256, True, False, eps=1e-30, gate=torch.rand(T, 1, device="cuda"), **kw)
+        _check(p, T, 256, True, False, gate=torch.rand(256, device="cuda"), **kw)
+
+
+@pytest.mark.parametrize("T", [12, 1300])
 def test_products_that_underflow(T):
     """Blocks whose second weights, gates or inputs lie many powers of two below the row's."""
     p = require_gpu()
