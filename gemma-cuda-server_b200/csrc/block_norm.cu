@@ -125,6 +125,32 @@ __device__ __forceinline__ V8 gate8(const NormParams& p, int row, int ch) {
     return g;
 }
 
+// Whether one of the lane's elements of a row, t = (y fg) w gate, is zero although none of its factors is (w: bf16, not NULL).
+template <Src Y>
+__device__ __noinline__ bool lost_row(const NormParams& p, int row, float fg, const void* y, const uint4* w) {
+    const bool g_col = p.a.gate && p.a.gate_col_stride;
+    bool any = false;
+#pragma unroll 1
+    for (int ch = threadIdx.x & 31; ch < p.a.H >> 3; ch += 32) {
+        const V8 n = load8<Y>(y, ch), m = unpack8(w[ch]), g = g_col ? gate8(p, row, ch) : fill8(1.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            any |= n.at(i) * fg * m.at(i) * g.at(i) == 0.f && n.at(i) != 0.f && m.at(i) != 0.f && g.at(i) != 0.f;
+    }
+    return any;
+}
+
+// Whether a chunk of zeros has an element where none of y, the weight (NULL = 1) and the gate is.
+template <Src Y>
+__device__ __noinline__ bool lost_chunk(const NormParams& p, int row, int ch, float g_row, const void* y) {
+    const V8 n = load8<Y>(y, ch), m = weight8(p.a.post_weight, ch);
+    const V8 g = p.a.gate && p.a.gate_col_stride ? gate8(p, row, ch) : fill8(g_row);
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) any |= n.at(i) != 0.f && m.at(i) != 0.f && g.at(i) != 0.f;
+    return any;
+}
+
 __device__ __forceinline__ float sum_sq(const V8& v) {
     float2 s = __fmul2_rn(v.p[0], v.p[0]);
 #pragma unroll
@@ -190,6 +216,14 @@ __device__ __forceinline__ float max_abs(const V8& v) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(fabsf(v.p[j].x), fabsf(v.p[j].y)));
     return m;
+}
+
+// Whether an element of both is not zero: a block of zeros is one of true zeros, or of products that underflowed.
+__device__ __forceinline__ bool both_nonzero(const V8& a, const V8& b) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) any |= a.at(i) != 0.f && b.at(i) != 0.f;
+    return any;
 }
 
 __device__ __forceinline__ void store_resid(const nvfp4b_block_norm_args& a, int row, int ch, const V8& r) {
@@ -370,7 +404,10 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                         s2 = __ffma2_rn(b, b, s2);
                     }
                 }
-                if constexpr (MX) sa += s2.x + s2.y;
+                if constexpr (MX) {
+                    sa += s2.x + s2.y;
+                    if (top[c] == 0.f && lost_chunk<Y>(p, row, ch, g_row.x, sy)) sa = __int_as_float(0x7F800000);   // wild
+                }
                 if (want_z) ss += sum_sq(r[c]);
             }
         } else {
@@ -443,7 +480,9 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                     const uint32_t up = cvt_e2m1x8(hi[0].x, hi[0].y, hi[1].x, hi[1].y, hi[2].x, hi[2].y, hi[3].x, hi[3].y);
                     const bool doubt = code[c] != up || byte[c] != mx_byte(__float_as_uint(fmaxf(zm - dm, 0.f))) ||
                                        top_bits >= 0x7F000000u ||
-                                       (top_bits != 0u && top_bits < 0x21800000u) ||  // below 2^-60
+                                       (top_bits < 0x21800000u &&                      // below 2^-60, or underflowed
+                                        (top_bits != 0u || (HAS_Y ? top[c] > 0.f && wm > 0.f
+                                                                  : ch < chunks && both_nonzero(load8<R>(sr, ch), w)))) ||
                                        !(all.x + all.y == all.x + all.y);
                     redo |= doubt ? 1u << c : 0u;
                 }
@@ -757,7 +796,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
             fgs = f * g_row * a.scale;
         }
         const float2 scale2 = make_float2(a.scale, a.scale);
-        float t_max = 0.f, st = 0.f;
+        float t_max = 0.f, t_min = 1.f, st = 0.f;                   // max |t|, the least of the chunks' max |t|, sum t^2
         SumSq ss;
         if constexpr (HAS_Y) {
             const float2 fgs2 = make_float2(fgs, fgs);
@@ -774,13 +813,15 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) r.p[j] = __ffma2_rn(v.p[j], scale2, t.p[j]);
+                if constexpr (MX) {
+                    st += sum_sq(t);
+                    const float m = max_abs(t);
+                    t_max = fmaxf(t_max, m);
+                    t_min = fminf(t_min, m);
+                }
                 *r_lo(ch) = make_float4(r.p[0].x, r.p[0].y, r.p[1].x, r.p[1].y);
                 *r_hi(ch) = make_float4(r.p[2].x, r.p[2].y, r.p[3].x, r.p[3].y);
                 ss.add(r);
-                if constexpr (MX) {
-                    st += sum_sq(t);
-                    t_max = fmaxf(t_max, max_abs(t));
-                }
             }
         } else {
 #pragma unroll 4
@@ -810,6 +851,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
         if (want_z) {
             const float sum = ss.total();
             if constexpr (MX && HAS_Y) {
+                if (t_min == 0.f && g_row != 0.f && lost_row<Y>(p, row, fgs, y_row(row), w_post))
+                    st = __int_as_float(0x7F800000);                // makes the row wild
                 st = warp_sum(st);
                 rel = st > 0.f ? fmaf(sqrtf(st / sum), kE, kE) : kE;
                 wild |= !(rel < 0x1p-12f);                          // also where sum = 0 < st: r cancelled altogether
@@ -826,7 +869,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
             for (int j = 0; j < 4; ++j) z.p[j] = __fmul2_rn(__fmul2_rn(r.p[j], f2), w.p[j]);
             return z;
         };
-        uint32_t row_max = 0, doubt = 0;                            // bit i: the chunk of loop step i is not proven
+        uint32_t row_max = 0, doubt = 0, zeros = 0;                 // bit i: the chunk of loop step i is not proven, is 0
         // r and z are stored at once, unless that would overwrite what a redo reads again
         const bool later = MX && p.in_place;
         if (!wild) {
@@ -878,7 +921,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
                     // also where the exponent is in doubt, or the values are near the ends of the range
                     const bool unsure = code != other || ((top ^ bot) & 0x7F800000u) != 0u ||
                                         top - 0x21800000u >= 0x7F000000u - 0x21800000u;
-                    doubt |= unsure && top != 0u ? 1u << i : 0u;
+                    doubt |= unsure ? 1u << i : 0u;
+                    zeros |= top == 0u ? 1u << i : 0u;              // unsure, too
                     // zeros that agree: the end that kept their sign (x - 0 of each, or x + x rel)
                     if (ok) code_row[ch] = HAS_Y ? code : other;
                     uint32_t w = ok ? ((field >> 23) - 2u) << (8 * ((lane & 15) >> 2)) : 0u;
@@ -886,6 +930,13 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
                     w |= __shfl_xor_sync(0xFFFFFFFFu, w, 8);
                     if ((lane & 15) == 0 && ch < p.chunks16) *reinterpret_cast<uint32_t*>(scale_row + 32 * ch) = w;
                 }
+            }
+        }
+        if constexpr (MX) {
+            for (; zeros; zeros &= zeros - 1) {                     // true zeros need no redo, products that underflowed do
+                const int ch = 32 * (__ffs(zeros) - 1) + lane;
+                if (ch >= chunks || !both_nonzero(HAS_Y ? r_chunk(ch) : load8<R>(sr, ch), unpack8(w_norm[ch])))
+                    doubt &= ~(zeros & (0u - zeros));
             }
         }
         doubt = __reduce_or_sync(0xFFFFFFFFu, doubt);               // from here on the same on every lane, as `wild` is

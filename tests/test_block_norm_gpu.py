@@ -394,7 +394,7 @@ def test_rows_whose_squares_underflow(T, eps, e):
 
 
 @pytest.mark.parametrize("T", [12, 1300])
-@pytest.mark.parametrize("y_exp,w_exp", [(-30, -108), (-30, -112), (-60, -84), (0, -126), (20, -126)])
+@pytest.mark.parametrize("y_exp,w_exp", [(-30, -108), (-30, -112), (-60, -84), (0, -126), (20, -126), (-10, -133)])
 def test_products_of_input_and_weight_that_underflow(T, y_exp, w_exp):
     """A block whose y post_weight needs bits below the smallest fp32, brought back by the second weights."""
     p = require_gpu()
