@@ -156,12 +156,14 @@ __device__ __noinline__ uint32_t geglu_block64(const uint16_t* gp, const uint16_
 
 // Whether estimates that have no relative bound matter: where -w nears the end of the fp32 range or h the subnormals,
 // |h| <= |g u| 2^-100, and such an element has code 0 (the smallest magnitude with another one is above top / 32) unless
-// the whole block is that small.
+// the whole block is that small.  From g = -1.5e13 down w and its bound are infinities: 0 * inf would make both ends of a
+// signed zero NaN, whose codes agree.
 __device__ __noinline__ bool geglu_tiny(const uint16_t* gp, const uint16_t* up, float top) {
     float tiny = 0.f;
 #pragma unroll 1
     for (int i = 0; i < 16; ++i) {
         const float g = __uint_as_float((uint32_t)gp[i] << 16), u = __uint_as_float((uint32_t)up[i] << 16);
+        if (g < -0x1p43f) return true;
         if (g != 0.f && u != 0.f) tiny = fmaxf(tiny, fmaxf(fabsf(g * u), 1.0f) * 0x1p-100f);
     }
     return tiny > top * 0x1p-6f;
@@ -171,8 +173,7 @@ __device__ __noinline__ bool geglu_tiny(const uint16_t* gp, const uint16_t* up, 
 // g * rcp(1 + ex2(-w)) * u is off by at most |h| e, e = max(-w, 1) 2^-22 + 2^-20: the roundings of w leave it 3.5 * 2^-24
 // off, so the exponential 2.5 |w| 2^-24, which for w > 0 enters through ex2(-w) / (1 + ex2(-w)) only (below 1 / w);
 // ex2.approx 2^-22, the sum, the reciprocal and the products add 9 * 2^-24, h - d and h + d the rest.  The .ftz forms flush
-// where w > 126 (the exponential adds nothing to 1) or w < -100 (no bound there, below).  From g = -1.5e13 down w is an
-// infinity, and so is e: 0 * e makes both ends NaN, whose codes agree, so those blocks are redone by the size of w.
+// where w > 126 (the exponential adds nothing to 1) or w < -100 (no bound there, above).
 template <bool WIDE>
 __global__ void __launch_bounds__(kMxThreads) mx_geglu_kernel(const uint16_t* __restrict__ x, long long ldx, int M,
                                                               int I, uint8_t* __restrict__ codes,
@@ -217,8 +218,7 @@ __global__ void __launch_bounds__(kMxThreads) mx_geglu_kernel(const uint16_t* __
         const float inv = __uint_as_float(0x80000000u - field);
         const float total = sum.x + sum.y;                             // NaN where an h is (no maximum shows it)
         bool redo = ((hi ^ lo) & 0x7F800000u) != 0u || hi >= 0x7F000000u || !(total == total);
-        if (p.ok && (w_min <= -100.f || hi < 0x12800000u))                                    // 2^-90
-            redo |= w_min < -0x1p127f || geglu_tiny(gp, gp + I, top);
+        if (p.ok && (w_min <= -100.f || hi < 0x12800000u)) redo |= geglu_tiny(gp, gp + I, top);   // 2^-90
         uint32_t c[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
