@@ -1074,33 +1074,56 @@ int dispatch_block_norm(NormParams& p, cudaStream_t s) {
 
 bool bad_rows(const void* p, int f32, long long ld) { return !aligned16(p) || (ld * (f32 ? 4 : 2)) % 16; }
 
-// T rows of `width` bytes, `pitch` bytes apart (p NULL: not there).
+// Memory that a call reads or writes: n runs of `width` bytes, `pitch` bytes apart (p NULL: not there); one run where
+// nothing lies between them.
 struct Region {
-    const void* p;
-    long long pitch, width;
+    long long p, pitch, width, n;
+    Region(const void* p_, long long width_, long long pitch_ = 0, long long n_ = 1)
+        : p((long long)reinterpret_cast<uintptr_t>(p_)), pitch(pitch_), width(width_), n(n_) {
+        if (n == 1 || pitch <= width) {
+            width += (n - 1) * pitch;
+            pitch = 0;
+            n = 1;
+        }
+    }
+    long long end() const { return p + (n - 1) * pitch + width; }
 };
 
-// Whether two regions share memory otherwise than row for row (`same` allowed) -- side by side in the same pitch they do not.
-bool clash(const Region& a, const Region& b, long long T, bool same) {
-    if (!a.p || !b.p) return false;
-    const long long pa = (long long)reinterpret_cast<uintptr_t>(a.p), pb = (long long)reinterpret_cast<uintptr_t>(b.p);
-    if (pa >= pb + (T - 1) * b.pitch + b.width || pb >= pa + (T - 1) * a.pitch + a.width) return false;
-    if (same && pa == pb && a.width == b.width && (T == 1 || a.pitch == b.pitch)) return false;
-    if (a.pitch != b.pitch || a.pitch <= 0) return true;
-    const long long d = ((pb - pa) % a.pitch + a.pitch) % a.pitch;
+// Whether a run of `a` meets the one run `b`.
+bool meets(const Region& a, const Region& b) {
+    const long long d = b.p - a.p - a.width, i = d < 0 ? 0 : a.pitch ? d / a.pitch + 1 : 1;   // the first that ends behind b.p
+    return i < a.n && a.p + i * a.pitch < b.p + b.width;
+}
+
+// Whether two regions share memory otherwise than run for run (`same` allowed) -- side by side in one pitch they do not; of
+// different pitches that interleave it is assumed.
+bool clash(const Region& a, const Region& b, bool same = false) {
+    if (!a.p || !b.p || a.p >= b.end() || b.p >= a.end()) return false;
+    if (same && a.p == b.p && a.width == b.width && a.pitch == b.pitch) return false;
+    if (b.n == 1) return meets(a, b);
+    if (a.n == 1) return meets(b, a);
+    if (a.pitch != b.pitch) return true;
+    const long long d = ((b.p - a.p) % a.pitch + a.pitch) % a.pitch;
     return d < a.width || d + b.width > a.pitch;
 }
 
+// Whether an output shares memory with another one, or with an input (resid_out and out may be resid or y themselves).
 bool clashes(const nvfp4b_block_norm_args& a) {
-    const auto rows = [&](const void* p, int f32, long long ld) { return Region{p, ld * (f32 ? 4 : 2), a.H * (f32 ? 4ll : 2ll)}; };
-    const Region in[] = {rows(a.resid, a.resid_f32, a.ld_resid), rows(a.y, a.y_f32, a.ld_y)};
-    const Region r = rows(a.resid_out, a.resid_out_f32, a.ld_resid_out), z = rows(a.out, 0, a.ld_out);
-    const Region c = {a.codes, a.H / 2, a.H / 2};
-    const Region g = a.gate_col_stride ? rows(a.gate, a.gate_f32, a.gate_row_stride) : Region{};
-    for (const Region& x : in)
-        if (clash(r, x, a.T, true) || clash(z, x, a.T, true) || clash(c, x, a.T, false)) return true;
-    return clash(r, z, a.T, false) || clash(r, c, a.T, false) || clash(z, c, a.T, false) || clash(r, g, a.T, false) ||
-           clash(z, g, a.T, false) || clash(c, g, a.T, false);
+    const auto rows = [&](const void* p, int f32, long long ld) { return Region(p, a.H * (f32 ? 4ll : 2ll), ld * (f32 ? 4 : 2), a.T); };
+    const long long gate_size = a.gate_f32 ? 4 : 2;
+    const Region out[] = {rows(a.resid_out, a.resid_out_f32, a.ld_resid_out), rows(a.out, 0, a.ld_out),
+                          Region(a.codes, (long long)a.T * (a.H / 2)),
+                          Region(a.scales, (long long)nvfp4b_mx_scale_buffer_bytes(a.T, a.H)), Region(a.amax, 4)};
+    const Region in[] = {rows(a.resid, a.resid_f32, a.ld_resid), rows(a.y, a.y_f32, a.ld_y), Region(a.post_weight, a.H * 2ll),
+                         Region(a.norm_weight, a.H * 2ll),
+                         Region(a.gate, a.gate_col_stride ? a.H * gate_size : gate_size, a.gate_row_stride * gate_size, a.T)};
+    for (int i = 0; i < 5; ++i) {
+        for (int j = 0; j < 5; ++j)
+            if (clash(out[i], in[j], i < 2 && j < 2)) return true;
+        for (int j = 0; j < i; ++j)
+            if (clash(out[i], out[j])) return true;
+    }
+    return false;
 }
 
 }  // namespace

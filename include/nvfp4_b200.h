@@ -193,9 +193,9 @@ int nvfp4b_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, 
  * input is read once and r and z are taken from the unrounded values of the step before.  fp32 sums; the MXFP4 codes and
  * scales are those of the float64 z.  *amax (zeroed by this call) is the maximum of the bf16 out, as nvfp4b_amax_bf16
  * would find it: out and amax are what nvfp4b_quantize_bf16 takes with a dynamic scale.
- * resid_out and out may each be resid or y themselves (same type and pitch); rows that share memory in any other way are
- * refused (NVFP4B_ERR_ARG), columns side by side in one buffer are not.  Rows are `ld_*` elements apart.  H % 8 == 0
- * (% 32 with codes). */
+ * resid_out and out may each be resid or y themselves (same type and pitch); an output that shares memory with an input
+ * or another output in any other way is refused (NVFP4B_ERR_ARG), columns side by side in one buffer are not.  Rows are
+ * `ld_*` elements apart.  H % 8 == 0 (% 32 with codes). */
 #define NVFP4B_BLOCK_NORM_MAX_H 16384
 
 typedef struct nvfp4b_block_norm_args {
