@@ -289,6 +289,20 @@ __device__ __forceinline__ double sum_sq64(const V8& v, bool wild) {
     return ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
 }
 
+// The root of r's mean of squares, to divide by: x times its reciprocal, corrected by the remainder, is the rounded quotient
+// (in signs that leave a zero its own).  Without the correction it is an ulp off where the quotient lies on a border, as
+// sqrt(H) does for a row's only element.  An infinite root divides to 0: reciprocal 0, no remainder.
+struct Rms64 {
+    double root, inv;
+    __device__ __forceinline__ explicit Rms64(double mean) : root(sqrt(mean)), inv(1.0 / root) {
+        if (inv == 0.0) root = 0.0;
+    }
+    __device__ __forceinline__ double divide(double x) const {
+        const double q = x * inv;
+        return fma(-fma(q, root, -x), inv, q);
+    }
+};
+
 // r of a chunk in float64, by the operations of its definition in their order (an exact zero keeps its sign); w = the post
 // weights of the chunk, fg = 1 / rms(y), times the gate unless it is per feature.
 template <Src Y, Src R>
@@ -507,7 +521,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
 #pragma unroll
                 for (int i = 0; i < 8; ++i) s = fma(v[i], v[i], s);
             }
-            const double f2 = rsqrt(block_sum(s, red64[1]) / a.H + (double)a.eps);
+            const Rms64 rms_r(block_sum(s, red64[1]) / a.H + (double)a.eps);
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
                 const int ch = tid + c * threads;
@@ -526,7 +540,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                     const V8 w = weight8(a.norm_weight, ch);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const double zz = v[i] * f2 * (double)w.at(i);
+                        const double zz = rms_r.divide(v[i]) * (double)w.at(i);
                         if (wild) {
                             ((i & 1) ? r[c].p[i >> 1].y : r[c].p[i >> 1].x) = (float)v[i];
                             ((i & 1) ? z[c].p[i >> 1].y : z[c].p[i >> 1].x) = (float)zz;
@@ -597,7 +611,7 @@ struct Row64 {
     const uint4* w_post;
     int row, chunks;
     bool has_v, g_col;
-    double fg, f, scale;
+    double fg, scale;
 
     __device__ __forceinline__ void r8(int ch, double (&r)[8]) const {
         const V8 x = load8<R>(v, ch);
@@ -645,7 +659,6 @@ struct Row64 {
         g_col = Y != kNone && p.a.gate && p.a.gate_col_stride;
         fg = Y != kNone && p.a.gate && !g_col ? (double)gate_at(p.a, row, 0) : 1.0;
         if (Y != kNone && p.a.post_norm) fg *= rsqrt(sum_sq<true>() / h + eps);
-        f = rsqrt(sum_sq<false>() / h + eps);
     }
 };
 
@@ -657,6 +670,7 @@ __device__ __noinline__ uint32_t redo_row64(const NormParams& p, int row, uint32
     const nvfp4b_block_norm_args& a = p.a;
     const int lane = threadIdx.x & 31;
     const Row64<Y, R> q(p, row, y, v, w_post);
+    const Rms64 rms_r(q.template sum_sq<false>() / (double)a.H + (double)a.eps);
     __syncwarp();                                                   // codes and scale words stored before come first
     uint32_t zmax = 0;
     int step = 0;
@@ -677,7 +691,7 @@ __device__ __noinline__ uint32_t redo_row64(const NormParams& p, int row, uint32
             if (wild && a.resid_out) store_resid(a, row, ch, s);    // in place: the lane has read its own chunk
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                z[k] = z[k] * q.f * (double)w.at(k);
+                z[k] = rms_r.divide(z[k]) * (double)w.at(k);
                 amax = z[k] != z[k] ? __longlong_as_double(0x7FF0000000000000ll) : fmax(amax, fabs(z[k]));
             }
 #pragma unroll

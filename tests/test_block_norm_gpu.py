@@ -434,3 +434,23 @@ def test_products_that_underflow(T):
             kw["post_weight"][224:240] *= 2.0 ** -110
         _check(p, T, H, True, False, **kw)
         _check(p, T, H, True, False, eps=0.0, **kw)
+
+
+@pytest.mark.parametrize("T", [20, 1300])
+@pytest.mark.parametrize("H", [64, 256, 1024, 4096])
+@pytest.mark.parametrize("dtype", [B, F])
+def test_rows_of_one_element(T, H, dtype):
+    """A lone element has z = sqrt(H) w, a power of two that the scale byte turns on, whatever its size and the roundings."""
+    p = require_gpu()
+    rng = np.random.default_rng(H)
+    x = torch.zeros(T, H, dtype=dtype, device="cuda")
+    at = torch.from_numpy(rng.integers(0, H, T)).cuda()
+    x[torch.arange(T), at] = torch.from_numpy(rng.normal(0, 1, T) * 2.0 ** rng.integers(-40, 40, T)).to(dtype).cuda()
+    w = torch.full((H,), 1.0, dtype=B, device="cuda")
+    for kw in (dict(resid=x), dict(y=x, post_norm=False), dict(y=x, post_norm=True), dict(y=x, post_weight=w, norm_weight=w),
+               dict(resid=x, y=x, post_norm=False), dict(resid=x, y=x, post_norm=True)):
+        got = p.block_norm(**kw, eps=0.0, mx=True)
+        z = torch.where(x != 0, torch.sign(x.double()) * H ** 0.5, 0.0)
+        ref = mx.quantize(_n(z))
+        byte, _ = mx.untile_scales(got.scales.cpu().numpy(), T, H)
+        assert np.array_equal(byte, ref[1]) and np.array_equal(got.codes.cpu().numpy(), ref[0])
