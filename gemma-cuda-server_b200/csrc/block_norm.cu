@@ -125,29 +125,20 @@ __device__ __forceinline__ V8 gate8(const NormParams& p, int row, int ch) {
     return g;
 }
 
-// Whether one of the lane's elements of a row, t = (y fg) w gate, is zero although none of its factors is (w: bf16, not NULL).
+// Whether an element of the chunks first, first + step ..., t = (y fg) w gate, is zero although none of its factors is (w: bf16,
+// NULL = ones).
 template <Src Y>
-__device__ __noinline__ bool lost_row(const NormParams& p, int row, float fg, const void* y, const uint4* w) {
+__device__ __noinline__ bool lost_row(const NormParams& p, int row, float fg, const void* y, const void* w, int first, int step) {
     const bool g_col = p.a.gate && p.a.gate_col_stride;
     bool any = false;
 #pragma unroll 1
-    for (int ch = threadIdx.x & 31; ch < p.a.H >> 3; ch += 32) {
-        const V8 n = load8<Y>(y, ch), m = unpack8(w[ch]), g = g_col ? gate8(p, row, ch) : fill8(1.f);
+    for (int ch = first; ch < p.a.H >> 3; ch += step) {
+        const V8 n = load8<Y>(y, ch), m = w ? unpack8(static_cast<const uint4*>(w)[ch]) : fill8(1.f);
+        const V8 g = g_col ? gate8(p, row, ch) : fill8(1.f);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             any |= n.at(i) * fg * m.at(i) * g.at(i) == 0.f && n.at(i) != 0.f && m.at(i) != 0.f && g.at(i) != 0.f;
     }
-    return any;
-}
-
-// Whether a chunk of zeros has an element where none of y, the weight (NULL = 1) and the gate is.
-template <Src Y>
-__device__ __noinline__ bool lost_chunk(const NormParams& p, int row, int ch, float g_row, const void* y) {
-    const V8 n = load8<Y>(y, ch), m = weight8(p.a.post_weight, ch);
-    const V8 g = p.a.gate && p.a.gate_col_stride ? gate8(p, row, ch) : fill8(g_row);
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) any |= n.at(i) != 0.f && m.at(i) != 0.f && g.at(i) != 0.f;
     return any;
 }
 
@@ -392,6 +383,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                 f = __frsqrt_rn(m);
             }
             const float2 fg = make_float2(f * g_row.x, f * g_row.y), scale = make_float2(a.scale, a.scale);
+            float least = 1.f;                           // of the chunks' A
             ss = 0.f;
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
@@ -420,10 +412,12 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                 }
                 if constexpr (MX) {
                     sa += s2.x + s2.y;
-                    if (top[c] == 0.f && lost_chunk<Y>(p, row, ch, g_row.x, sy)) sa = __int_as_float(0x7F800000);   // wild
+                    least = fminf(least, top[c]);
                 }
                 if (want_z) ss += sum_sq(r[c]);
             }
+            if (MX && least == 0.f && g_row.x != 0.f && lost_row<Y>(p, row, fg.x, sy, a.post_weight, tid, threads))
+                sa = __int_as_float(0x7F800000);         // makes the row wild
         } else {
             const float2 scale = make_float2(a.scale, a.scale);
 #pragma unroll
@@ -865,7 +859,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
         if (want_z) {
             const float sum = ss.total();
             if constexpr (MX && HAS_Y) {
-                if (t_min == 0.f && g_row != 0.f && lost_row<Y>(p, row, fgs, y_row(row), w_post))
+                if (t_min == 0.f && g_row != 0.f && lost_row<Y>(p, row, fgs, y_row(row), w_post, lane, 32))
                     st = __int_as_float(0x7F800000);                // makes the row wild
                 st = warp_sum(st);
                 rel = st > 0.f ? fmaf(sqrtf(st / sum), kE, kE) : kE;
