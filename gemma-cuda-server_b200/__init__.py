@@ -429,8 +429,8 @@ def mx_dequantize(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype 
 def mx_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
             out: torch.Tensor | None = None, out_kind: int = OUT_BF16_ROWMAJOR, alpha: float = 1.0,
             stream=None) -> torch.Tensor:
-    """D = alpha * A @ B^T on the MXFP4 tensor cores.  A: codes [M, K/2]; B: codes [N, K/2]; tile-layout scales.  D is
-    [M, N] bf16 or fp32 (rows may be strided), or fp32 [N, M] with OUT_F32_COLMAJOR, as in ``gemm``."""
+    """D = alpha * A @ B^T on the MXFP4 tensor cores.  A: codes [M, K/2]; B: codes [N, K/2]; tile-layout scales (zero
+    in the padding, as every producer here leaves them).  D is [M, N] bf16 or fp32 (rows may be strided), or fp32 [N, M] with OUT_F32_COLMAJOR, as in ``gemm``."""
     M, K, dev = _mx_operand("mx_gemm: a", a, a_scales)
     N, kb, _ = _mx_operand("mx_gemm: b", b, b_scales, dev)
     if kb != K:
@@ -469,7 +469,8 @@ def block_norm(resid: torch.Tensor | None = None, norm_weight: torch.Tensor | No
     normalised (default: with a post_weight); gate: bf16 or fp32, [H] per feature, [T, 1] per token or [T, H].
     z goes to `out` (bf16 [T, H]; with `amax`, fp32 [1], its max |z|) and / or to MXFP4 `codes` and `scales` (mx=True
     allocates them); with a norm_weight and neither, to a new `out`.  Where nothing is asked for but y is given, r goes to
-    a new resid_out of resid's type (or y's).  resid_out and out may be resid or y themselves, of the same type and pitch."""
+    a new resid_out of resid's type (or y's).  resid_out and out may be resid or y themselves, of the same type and pitch;
+    an output that shares memory with anything else is refused."""
     x = resid if resid is not None else y
     if x is None:
         raise ValueError("block_norm: resid or y is needed")

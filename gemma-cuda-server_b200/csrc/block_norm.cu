@@ -3,7 +3,8 @@
 // r is written as the new residual; z as bf16 (with its max |.|, the dynamic scale of an NVFP4 quantiser) and/or as MXFP4
 // codes and scales.  Each input is read once and each output written once; DRAM bounds it at prefill sizes.
 //
-// Persistent CTAs, one row at a time, 8 consecutive elements per thread and chunk.  The rows of y and resid come by
+// Two kernels: a row per warp from a few rows per SM on (block_norm_rows_kernel, below), else a row per CTA.  This one:
+// persistent CTAs, one row at a time, 8 consecutive elements per thread and chunk.  The rows of y and resid come by
 // bulk copies into a ring of two shared-memory stages, so the next row is on its way while this one goes through its
 // two or three block-wide barriers (a first version with a CTA per row and loads into registers spent its time
 // waiting: 148 us for 8192 x 2816 bf16 with a gate to MXFP4).  NCH chunks per thread: 2 or 4 at many rows (small
@@ -711,7 +712,7 @@ __device__ __noinline__ uint32_t redo_row64(const NormParams& p, int row, uint32
 // copies) is paid by one warp instead of all warps of a CTA.  Each warp owns one row buffer in shared memory; the weights
 // lie there once per CTA; the next row is prefetched into L2 meanwhile.  Pass 1: sum of y^2.  Pass 2: r, written over
 // the chunk's own y and resid, and the sums of r^2 and t^2 (t = scale * gate * n).  Pass 3: outputs.  Short code at any
-// H, and 16 warps per SM hide each other's latencies (two stages and 8 warps: 92 against 70 us at 8192 x 2816).
+// H, and 16 warps per SM hide each other's latencies (two stages and 8 warps took a third longer at 8192 x 2816).
 //
 // Bounds: a chunk's sum of squares is off by 4 u of itself, its compensated sum over the row's chunks and the float64
 // tree by less than 0.1 u more, 1 / rms by 4.5 u; t by 8.5 u |t|, r by that + u |r|, and z (the rounding of z - d and
@@ -720,7 +721,7 @@ __device__ __noinline__ uint32_t redo_row64(const NormParams& p, int row, uint32
 // T = max |t| of the lane's chunks, Z = max |z| of the chunk (one d serves its 8 elements); without y by E |z|.  One row
 // in sixteen at 2816 elements holds an element that near to a border.  Its redo takes a warp nearly as long as the row
 // did, most of it conversions to float64, so the warps of a CTA take their rows from a common count (8192 x 2816 with a
-// gate: 55 us, 76 us with a fixed share of the rows for each warp).
+// gate: 55 us, 40% more with a fixed share of the rows for each warp).
 template <Src Y, Src R, bool MX>
 __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(const __grid_constant__ NormParams p) {
     using namespace sm100;
@@ -1006,10 +1007,10 @@ int raise_smem(const void* kernel, std::atomic<bool> (&ready)[64]) {   // once p
 
 // The row kernel's launch; `fits` false (nothing launched) where a row has more loop steps than a 32-bit mask, or where the
 // row buffers that shared memory holds are too few.  With y and codes, which is the most to compute, six do (4096 wide,
-// fp32 y and resid, 8192 rows: 122 us, 151 by CTAs; five, 8192 wide bf16: 238 and 243, but 1500 rows 69 and 53), if the
+// fp32 y and resid, 8192 rows: 122 us, 163 by CTAs; five, 8192 wide bf16: 243 and 248, but 1500 rows 74 and 58), if the
 // scale is positive: it goes into the sum's terms there, which a scale below or at zero would give zeros of another sign.  Else
-// all sixteen, or eight and four rounds of rows (4096 wide, bf16 y and resid to bf16, twelve warps: 8192 rows 55 us, 60 by
-// CTAs; 4096 rows 35 and 32).
+// all sixteen, or eight and four rounds of rows (4096 wide, bf16 y and resid to bf16, twelve warps: 8192 rows 55 us, 62 by
+// CTAs; 4096 rows 35 and 34).
 template <Src Y, Src R, bool MX>
 int launch_block_norm_rows(NormParams& p, cudaStream_t s, bool& fits) {
     const auto kernel = block_norm_rows_kernel<Y, R, MX>;
@@ -1050,12 +1051,12 @@ int launch_block_norm(NormParams& p, cudaStream_t s) {
     return launch_k(kernel, dim3((unsigned)grid), dim3(threads), smem, s, p);
 }
 
-// From kRowKernelRows rows per SM on a warp per row, where its buffers fit (900 x 2816 with y to MXFP4 16.1 us, 19.6 by
-// CTAs; 700 rows 12.5 that way, 741 by warps 16.2); not with an fp32 y and no codes, where there is little to compute and a
-// row fills much shared memory (2900 x 2816 24.7 us by CTAs, 30.1 by warps).  Below a CTA per row: one chunk per thread,
-// the shortest path through a row, as far as the rows make two rounds (64 x 2816 with y to MXFP4 6.2 us); then two, for more
-// CTAs per SM (512 x 2816 fp32 to bf16 6.1 us, 6.8 with four; 739 x 4096 10.8 and 12.2), or with y and codes, where the
-// threads compute most, four (600 x 2816 12.1 us, 14.8 with two).
+// From kRowKernelRows rows per SM on a warp per row, where its buffers fit (900 x 2816 with y to MXFP4 16.3 us, 21.1 by
+// CTAs; 700 rows 16.0 and 13.2, 741 rows, where the switch is, 16.0 and 13.3); not with an fp32 y and no codes, where there is
+// little to compute and a row fills much shared memory (2900 x 2816 26.6 us by CTAs, 30.2 by warps).  Below a CTA per row: one
+// chunk per thread, the shortest path through a row, as far as the rows make two rounds (64 x 2816 with y to MXFP4 6.2 us);
+// then two, for more CTAs per SM (512 x 2816 fp32 to bf16 6.3 us, 7.2 with four; 739 x 4096 bf16 9.1 and 11.7), or with y and
+// codes, where the threads compute most, four (600 x 2816 12.6 us, 13.8 with two).
 constexpr int kRowKernelRows = 5;
 
 template <Src Y, Src R, bool MX>

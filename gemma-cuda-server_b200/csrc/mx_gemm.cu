@@ -26,8 +26,8 @@ struct MxGemm {
 
 // Epilogue of the CTA-pair tiles, which compute D^T = B A^T: a thread holds 32 columns of one row of the tile, so the lanes'
 // elements lie together in row-major D and each is stored from its register, 64 or 128 bytes of a row per instruction, at
-// any pitch.  The address goes up by additions: with a product for each element 4096 x 7000, K = 512 fp32 took 40.5 us, 27.3
-// so; through a swizzled tile in shared memory to 16 bytes per lane 31.1 (bf16 29.2, 25.9 so).
+// any pitch.  The address goes up by additions: with a product for each element 4096 x 7000, K = 512 fp32 took 48% longer;
+// through a swizzled tile in shared memory to 16 bytes per lane 14% (bf16 13%).
 template <typename T>
 struct MxEpi {
     T* d;
@@ -83,7 +83,7 @@ int mx_core_params(const MxGemm& g, CoreParams& cp) {
 //   warp 1      TMEM owner and MMA issuer
 //   warps 2..   epilogue, TMEM lane quadrant warp % 4: a thread holds one column n of D, 16 rows at a time.  Eight warps from
 //               32 rows on, two to a quadrant: a warp's own instructions are what the epilogue takes (512 x 2816,
-//               K = 2112 8.9 us with four, 8.4 with eight, no gain with sixteen)
+//               K = 2112 8.3 us with four, 7.9 with eight, no gain with sixteen)
 //   last warp   scale copies (issued by the MMA thread they made a K-tile take 1330 cycles)
 template <int NT_>
 struct SkinnyCfg {
@@ -130,7 +130,7 @@ __device__ __forceinline__ void skinny_store(const SkinnyParams& p, int m, int n
 
 // One warp stores rows m0.. (16 of them, `rows` exist) x columns n0.. (32) of D; lane = column in r.  Row-major a lane
 // stores its own column, row by row: the lanes' elements lie together, at any pitch (turned around in shared memory to 16
-// bytes per lane 8.4 against 7.9 us at 512 x 2816, K = 2112, and 10.7 against 9.5 at 128 x 65536, K = 256).  Column-major
+// bytes per lane 512 x 2816, K = 2112 took 6% longer and 128 x 65536, K = 256 13%).  Column-major
 // the rows are turned around in `t`.
 template <int OUT>
 __device__ __forceinline__ void skinny_store16(const SkinnyParams& p, int m0, int rows, int n0, const uint32_t (&r)[16],
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 1)
 
 // The CTAs that K is split over.  A split saves a CTA k_tiles (1 - 1/S) K-tiles of about 0.27 us and costs the meeting of
 // the partial sums, which grows with the tile's rows and is twice as dear column-major (N = 2816: 16 rows, K = 2816, S = 6
-// 5.1 against 7.0 us unsplit; 128 rows 8.0 and 8.3; K = 704, S = 3 4.9 and 4.5, 7.1 and 5.7), so it is taken from 3 +
+// 5.2 against 7.3 us unsplit; 128 rows 8.0 and 8.4; K = 704, S = 3 5.0 and 4.6, 7.1 and 5.7), so it is taken from 3 +
 // NT / 32 saved K-tiles on, and only as far as all clusters are resident at once (24 clusters of 6 are not: 14.4 us
 // against 8.4 with 4).
 template <int NT>
@@ -473,8 +473,8 @@ MxGemm swapped(const MxGemm& g) { return {g.b, g.b_sf, g.a, g.a_sf, g.alpha, g.N
 // Narrow tiles (128 x 128 above 64 rows) or CTA pairs (256 x 256)?  A round of narrow tiles takes about 0.42 us for each
 // K-tile and 0.4 us, 1.3 at least (the stores of one tile under the products of the next); a round of pairs 0.42 us for
 // each K-tile and 1.9 (one accumulator, so the stores are not hidden).  Narrow wins with few K-tiles, with one round, and
-// where the pairs' last round is nearly empty (1024 x 4736, K = 704 7.8 against 10.2 us; 4096 x 7000, K = 512 21.6 and
-// 25.9; K = 1408 37.6 and 34.6; 512 x 8448, K = 2816 13.6 and 11.0).
+// where the pairs' last round is nearly empty (1024 x 4736, K = 704 7.8 against 10.2 us; 4096 x 7000, K = 512 22.3 and
+// 26.2; K = 1408 38.0 and 34.8; 512 x 8448, K = 2816 14.2 and 11.5).
 bool narrow_tiles(int M, int N, int K) {
     const long long sms = sm_count(), pairs = sms / 2, kt = (K + 255) / 256;
     const long long rn = ((M + 127) / 128 * ((N + 127ll) / 128) + sms - 1) / sms;

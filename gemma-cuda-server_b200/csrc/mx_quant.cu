@@ -308,8 +308,8 @@ __global__ void __launch_bounds__(kMxThreads) mx_dequantize_kernel(const uint8_t
 
 struct MxGrid { uint32_t tile_cols, items; unsigned blocks; };
 
-// A warp per item, grid-stride over at most `per_sm` blocks per SM.  8192 x 2816: quantise 13.8 us at 16 and 14.9 at 8,
-// dequantise 10.3 and 10.6; the gated quantiser, which computes more per item, 12.4 us at 8 and 12.9 at 16 (4096 x 2112).
+// A warp per item, grid-stride over at most `per_sm` blocks per SM.  8192 x 2816: quantise 12.4 us at 16 and 13.5 at 8,
+// dequantise 12.6 and 12.7; the gated quantiser, which computes more per item, 11.6 us at 8 and 12.2 at 16 (4096 x 2112).
 unsigned mx_blocks(long long items, int per_sm) {
     const long long b = (items + kMxThreads / 32 - 1) / (kMxThreads / 32), cap = (long long)sm_count() * per_sm;
     return (unsigned)(b < cap ? b : cap);

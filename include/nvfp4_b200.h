@@ -179,7 +179,9 @@ int nvfp4b_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int M, int
 
 /* D = alpha * A @ B^T, A [M, K] and B [N, K] in MXFP4 (K-major codes, tile-layout scales), fp32 accumulation on the
  * tensor cores (tcgen05 kind::mxf4), out_kind and ldd as for nvfp4b_gemm.  Any M, N >= 1; operands and d 16-byte
- * aligned.  Deterministic: the same call gives the same bits. */
+ * aligned.  The scale bytes of padding blocks must be zero, as every producer here leaves them (K % 64 == 32: the last
+ * tensor-core step reads one, against codes of zero, and an 0xFF there would make its row or column NaN).
+ * Deterministic: the same call gives the same bits. */
 int nvfp4b_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, const uint8_t* b_scales, float alpha,
                    int M, int N, int K, void* d, int out_kind, long long ldd, void* stream);
 
@@ -191,7 +193,7 @@ int nvfp4b_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, 
  * with rms(x; eps) = x / sqrt(mean(x^2) + eps) over the H elements of a row (the reference's rmsnorm,
  * kernels/elementwise.cu:10-22, and the post-norms, residual and layer_scalar of moe(), src/forward.cu:546-551).  Every
  * input is read once and r and z are taken from the unrounded values of the step before.  fp32 sums; the MXFP4 codes and
- * scales are those of the float64 z.  *amax (zeroed by this call) is the maximum of the bf16 out, as nvfp4b_amax_bf16
+ * scales are those of the float64 z (where 1 / rms(r) and an element's two weights make less than 2^60).  *amax (zeroed by this call) is the maximum of the bf16 out, as nvfp4b_amax_bf16
  * would find it: out and amax are what nvfp4b_quantize_bf16 takes with a dynamic scale.
  * resid_out and out may each be resid or y themselves (same type and pitch); an output that shares memory with an input
  * or another output in any other way is refused (NVFP4B_ERR_ARG), columns side by side in one buffer are not.  Rows are
