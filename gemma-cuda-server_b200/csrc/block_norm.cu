@@ -126,20 +126,26 @@ __device__ __forceinline__ V8 gate8(const NormParams& p, int row, int ch) {
     return g;
 }
 
-// Whether an element of the chunks first, first + step ..., t = (y fg) w gate, is zero although none of its factors is (w: bf16,
-// NULL = ones).
-template <Src Y>
-__device__ __noinline__ bool lost_row(const NormParams& p, int row, float fg, const void* y, const void* w, int first, int step) {
-    const bool g_col = p.a.gate && p.a.gate_col_stride;
+// Whether an element of both is not zero.
+__device__ __forceinline__ bool both_nonzero(const V8& a, const V8& b) {
     bool any = false;
-#pragma unroll 1
-    for (int ch = first; ch < p.a.H >> 3; ch += step) {
-        const V8 n = load8<Y>(y, ch), m = w ? unpack8(static_cast<const uint4*>(w)[ch]) : fill8(1.f);
-        const V8 g = g_col ? gate8(p, row, ch) : fill8(1.f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            any |= n.at(i) * fg * m.at(i) * g.at(i) == 0.f && n.at(i) != 0.f && m.at(i) != 0.f && g.at(i) != 0.f;
-    }
+    for (int i = 0; i < 8; ++i) any |= a.at(i) != 0.f && b.at(i) != 0.f;
+    return any;
+}
+
+// Blocks of zeros: true ones, or products that underflowed.  Such a product is below 2^-149, so it matters (the least border is
+// 2^-129) only where the factors behind it make more than this: 1 / rms(r) and a second weight.
+constexpr float kZeroFactors = 0x1p18f;
+
+// Whether a chunk whose gate * n is zero has an element with y, weight (NULL = ones) and gate all nonzero.
+template <Src Y>
+__device__ __noinline__ bool lost_product(const NormParams& p, int row, int ch, float g_row, const void* y, const void* w) {
+    const V8 n = load8<Y>(y, ch), m = w ? unpack8(static_cast<const uint4*>(w)[ch]) : fill8(1.f);
+    const V8 g = p.a.gate && p.a.gate_col_stride ? gate8(p, row, ch) : fill8(g_row);
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) any |= n.at(i) != 0.f && m.at(i) != 0.f && g.at(i) != 0.f;
     return any;
 }
 
@@ -210,14 +216,6 @@ __device__ __forceinline__ float max_abs(const V8& v) {
     return m;
 }
 
-// Whether an element of both is not zero: a block of zeros is one of true zeros, or of products that underflowed.
-__device__ __forceinline__ bool both_nonzero(const V8& a, const V8& b) {
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) any |= a.at(i) != 0.f && b.at(i) != 0.f;
-    return any;
-}
-
 __device__ __forceinline__ void store_resid(const nvfp4b_block_norm_args& a, int row, int ch, const V8& r) {
     if (a.resid_out_f32) {
         float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.resid_out) + row * a.ld_resid_out) + 2 * ch;
@@ -249,7 +247,8 @@ __device__ __forceinline__ void zero_padding_rows(const NormParams& p) {
 // The float64 redo of a row: conversions, at an eighth of the fp32 rate, are what it costs.  The product of two bf16 values
 // is exact in fp32, but for underflow and overflow, and then one conversion serves both.  Squares: only a `wild` row holds
 // any whose underflow or overflow counts in the sum.  y post_weight: such a product may be all that an element is made of,
-// so chunks with one that is 0 or below 2^-130 (16 bits end at 2^-149 from 2^-134 down), or infinite, go the long way.
+// so chunks with one below 2^-130 (16 bits end at 2^-149 from 2^-134 down) of factors that are not 0, or infinite, go the
+// long way.
 template <Src Y>
 __device__ __forceinline__ void weighted64(const V8& y, const V8& w, double (&t)[8]) {
     bool exact = Y == kBf16;
@@ -261,7 +260,12 @@ __device__ __forceinline__ void weighted64(const V8& y, const V8& w, double (&t)
             lo = fminf(lo, q);
             hi = fmaxf(hi, q);
         }
-        exact = lo > 0x1p-130f && hi < __int_as_float(0x7F800000);
+        exact = hi < __int_as_float(0x7F800000);
+        if (lo <= 0x1p-130f) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                exact &= fabsf(y.at(i) * w.at(i)) > 0x1p-130f || y.at(i) == 0.f || w.at(i) == 0.f;
+        }
     }
     if (exact) {
 #pragma unroll
@@ -384,7 +388,6 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                 f = __frsqrt_rn(m);
             }
             const float2 fg = make_float2(f * g_row.x, f * g_row.y), scale = make_float2(a.scale, a.scale);
-            float least = 1.f;                           // of the chunks' A
             ss = 0.f;
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
@@ -411,14 +414,9 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                         s2 = __ffma2_rn(b, b, s2);
                     }
                 }
-                if constexpr (MX) {
-                    sa += s2.x + s2.y;
-                    least = fminf(least, top[c]);
-                }
+                if constexpr (MX) sa += s2.x + s2.y;
                 if (want_z) ss += sum_sq(r[c]);
             }
-            if (MX && least == 0.f && g_row.x != 0.f && lost_row<Y>(p, row, fg.x, sy, a.post_weight, tid, threads))
-                sa = __int_as_float(0x7F800000);         // makes the row wild
         } else {
             const float2 scale = make_float2(a.scale, a.scale);
 #pragma unroll
@@ -451,6 +449,11 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
             const float m = fmaf(ss, p.inv_h, a.eps);
             wild |= !mean_ok(m);
             f = __frsqrt_rn(m);
+            auto lost_zeros = [&](int c, int ch, float wm, const V8& w) {        // chunk c, of a block of zeros
+                if constexpr (!HAS_Y) return ch < chunks && both_nonzero(load8<R>(sr, ch), w);
+                else if (top[c] > 0.f) return wm > 0.f;
+                else return fmaxf(f, 1.f) * wm > kZeroFactors && lost_product<Y>(p, row, ch, g_row.x, sy, a.post_weight);
+            };
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
                 const int ch = tid + c * threads;
@@ -489,9 +492,8 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                     const uint32_t up = cvt_e2m1x8(hi[0].x, hi[0].y, hi[1].x, hi[1].y, hi[2].x, hi[2].y, hi[3].x, hi[3].y);
                     const bool doubt = code[c] != up || byte[c] != mx_byte(__float_as_uint(fmaxf(zm - dm, 0.f))) ||
                                        top_bits >= 0x7F000000u ||
-                                       (top_bits < 0x21800000u &&                      // below 2^-60, or underflowed
-                                        (top_bits != 0u || (HAS_Y ? top[c] > 0.f && wm > 0.f
-                                                                  : ch < chunks && both_nonzero(load8<R>(sr, ch), w)))) ||
+                                       (top_bits < 0x21800000u &&                      // below 2^-60, or lost
+                                        (top_bits != 0u || lost_zeros(c, ch, wm, w))) ||
                                        !(all.x + all.y == all.x + all.y);
                     redo |= doubt ? 1u << c : 0u;
                 }
@@ -805,7 +807,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
             fgs = f * g_row * a.scale;
         }
         const float2 scale2 = make_float2(a.scale, a.scale);
-        float t_max = 0.f, t_min = 1.f, st = 0.f;                   // max |t|, the least of the chunks' max |t|, sum t^2
+        float t_max = 0.f, st = 0.f;
         SumSq ss;
         if constexpr (HAS_Y) {
             const float2 fgs2 = make_float2(fgs, fgs);
@@ -824,9 +826,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
                 for (int j = 0; j < 4; ++j) r.p[j] = __ffma2_rn(v.p[j], scale2, t.p[j]);
                 if constexpr (MX) {
                     st += sum_sq(t);
-                    const float m = max_abs(t);
-                    t_max = fmaxf(t_max, m);
-                    t_min = fminf(t_min, m);
+                    t_max = fmaxf(t_max, max_abs(t));
                 }
                 *r_lo(ch) = make_float4(r.p[0].x, r.p[0].y, r.p[1].x, r.p[1].y);
                 *r_hi(ch) = make_float4(r.p[2].x, r.p[2].y, r.p[3].x, r.p[3].y);
@@ -860,8 +860,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
         if (want_z) {
             const float sum = ss.total();
             if constexpr (MX && HAS_Y) {
-                if (t_min == 0.f && g_row != 0.f && lost_row<Y>(p, row, fgs, y_row(row), w_post, lane, 32))
-                    st = __int_as_float(0x7F800000);                // makes the row wild
                 st = warp_sum(st);
                 rel = st > 0.f ? fmaf(sqrtf(st / sum), kE, kE) : kE;
                 wild |= !(rel < 0x1p-12f);                          // also where sum = 0 < st: r cancelled altogether
@@ -942,10 +940,15 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
             }
         }
         if constexpr (MX) {
-            for (; zeros; zeros &= zeros - 1) {                     // true zeros need no redo, products that underflowed do
-                const int ch = 32 * (__ffs(zeros) - 1) + lane;
-                if (ch >= chunks || !both_nonzero(HAS_Y ? r_chunk(ch) : load8<R>(sr, ch), unpack8(w_norm[ch])))
-                    doubt &= ~(zeros & (0u - zeros));
+            if (fmaxf(f, 1.f) * wm <= kZeroFactors) {
+                doubt &= ~zeros;
+            } else {
+                for (; zeros; zeros &= zeros - 1) {
+                    const int ch = 32 * (__ffs(zeros) - 1) + lane;
+                    bool lost = ch < chunks && both_nonzero(HAS_Y ? r_chunk(ch) : load8<R>(sr, ch), unpack8(w_norm[ch]));
+                    if constexpr (HAS_Y) lost = lost || (ch < chunks && lost_product<Y>(p, row, ch, g_row, y_row(row), w_post));
+                    if (!lost) doubt &= ~(zeros & (0u - zeros));
+                }
             }
         }
         doubt = __reduce_or_sync(0xFFFFFFFFu, doubt);               // from here on the same on every lane, as `wild` is
