@@ -159,10 +159,12 @@ __device__ __noinline__ uint32_t geglu_block64(const uint16_t* gp, const uint16_
 // the whole block is that small.  From g = -1.5e13 down w and its bound are infinities: 0 * inf would make both ends of a
 // signed zero NaN, whose codes agree.
 __device__ __noinline__ bool geglu_tiny(const uint16_t* gp, const uint16_t* up, float top) {
+    const Raw32 rg = load32<false>(gp), ru = load32<false>(up);
     float tiny = 0.f;
-#pragma unroll 1
+#pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const float g = __uint_as_float((uint32_t)gp[i] << 16), u = __uint_as_float((uint32_t)up[i] << 16);
+        const float g = (i & 1) ? bf16hi(rg.w[i >> 1]) : bf16lo(rg.w[i >> 1]);
+        const float u = (i & 1) ? bf16hi(ru.w[i >> 1]) : bf16lo(ru.w[i >> 1]);
         if (g < -0x1p43f) return true;
         if (g != 0.f && u != 0.f) tiny = fmaxf(tiny, fmaxf(fabsf(g * u), 1.0f) * 0x1p-100f);
     }
@@ -230,7 +232,9 @@ __global__ void __launch_bounds__(kMxThreads) mx_geglu_kernel(const uint16_t* __
                 b[j] = __ffma2_rn(v, d, v);
             }
             c[q] = cvt_e2m1x8(a[0].x, a[0].y, a[1].x, a[1].y, a[2].x, a[2].y, a[3].x, a[3].y);
-            redo |= c[q] != cvt_e2m1x8(b[0].x, b[0].y, b[1].x, b[1].y, b[2].x, b[2].y, b[3].x, b[3].y);
+            const uint32_t hi_end = cvt_e2m1x8(b[0].x, b[0].y, b[1].x, b[1].y, b[2].x, b[2].y, b[3].x, b[3].y);
+            redo |= ((c[q] ^ hi_end) & 0x77777777u) != 0u;             // a relative bound leaves no doubt about signs, and
+            c[q] = hi_end;                                             // h + d keeps that of a zero
         }
         redo |= __shfl_xor_sync(0xFFFFFFFFu, (int)redo, 1) != 0;      // both threads of a block, on every lane
         redo &= p.ok;

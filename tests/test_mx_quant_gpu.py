@@ -185,3 +185,17 @@ def test_geglu_masked_gates():
     gate[::7, ::5] = torch.finfo(torch.bfloat16).min
     want = mx.quantize(mx.geglu(gate.double().numpy(), up.double().numpy()))
     _check(*_run(p.mx_geglu_quantize, torch.cat([gate, up], 1).cuda(), 150, 704), want, 150, 704)
+
+
+def test_geglu_signed_zeros():
+    """Zeros of either sign among ordinary values, in gate, up or both, and whole rows of them: the sign of h on a code of zero."""
+    p = require_gpu()
+    g = torch.Generator().manual_seed(6)
+    gate, up = ((1.5 * torch.randn(200, 704, generator=g)).bfloat16() for _ in range(2))
+    for t, s in ((gate, 0), (up, 1)):
+        r = torch.rand(200, 704, generator=g)
+        t[r < 0.05], t[(r > 0.05) & (r < 0.1)] = 0.0, -0.0
+        t[190 + s], t[193 + s], t[196:, s::2] = 0.0, -0.0, 0.0
+    gate[180:184], up[180:184] = 0.0, 0.0
+    want = mx.quantize(mx.geglu(gate.double().numpy(), up.double().numpy()))
+    _check(*_run(p.mx_geglu_quantize, torch.cat([gate, up], 1).cuda(), 200, 704), want, 200, 704)
