@@ -194,8 +194,8 @@ int nvfp4b_mx_gemm(const uint8_t* a, const uint8_t* a_scales, const uint8_t* b, 
  * kernels/elementwise.cu:10-22, and the post-norms, residual and layer_scalar of moe(), src/forward.cu:546-551).  Every
  * input is read once and r and z are taken from the unrounded values of the step before.  fp32 sums; the MXFP4 codes and
  * scales are those of the float64 z (where 1 / rms(r) and an element's two weights make less than 2^60; a code of zero may
- * have the other sign where |gate * n| is below 2^-149).  *amax (zeroed by this call) is the maximum of the bf16 out, as nvfp4b_amax_bf16
- * would find it: out and amax are what nvfp4b_quantize_bf16 takes with a dynamic scale.
+ * have the other sign where |gate * n| is below 2^-149).  *amax (zeroed by this call) is the maximum of the bf16 out, as
+ * nvfp4b_amax_bf16 would find it: out and amax are what nvfp4b_quantize_bf16 takes with a dynamic scale.
  * resid_out and out may each be resid or y themselves (same type and pitch); an output that shares memory with an input
  * or another output in any other way is refused (NVFP4B_ERR_ARG), columns side by side in one buffer are not.  Rows are
  * `ld_*` elements apart.  H % 8 == 0 (% 32 with codes). */
