@@ -20,8 +20,9 @@
 //
 // Products are taken as (x f) w, f = 1 / rms(x): |x f| is at most sqrt(H), so what overflows is an overflow of the result,
 // while w f may leave fp32 at either end for finite values (w = 2^121 over rows of 2^-14 gave NaN for their zeros).  What
-// underflows is off by 2^-150 times the factors behind it; a block is redone where its maximum is below 2^-60, beside
-// which that does not count as long as 1 / rms(r) and the two weights of an element make less than 2^60.
+// underflows is off by 2^-150 times the factors behind it (a row whose gate / rms(y) does is redone); a block is redone where
+// its maximum is below 2^-60, beside which that does not count as long as 1 / rms(r) and the two weights of an element make
+// less than 2^60.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -134,16 +135,13 @@ __device__ __forceinline__ bool both_nonzero(const V8& a, const V8& b) {
     return any;
 }
 
-// Blocks of zeros: true ones, or products that underflowed.  Such a product is below 2^-149, so it matters (the least border is
-// 2^-129) only where the factors behind it make more than this: 1 / rms(r) and a second weight.  Below, a code of 0 may have the
-// sign of the rounded product and not of the product: looking at every block of zeros took 10% more where half the rows are.
-constexpr float kZeroFactors = 0x1p18f;
-
 // Whether a chunk whose gate * n is zero has an element with y, weight (NULL = ones) and gate all nonzero.
 template <Src Y>
 __device__ __noinline__ bool lost_product(const NormParams& p, int row, int ch, float g_row, const void* y, const void* w) {
-    const V8 n = load8<Y>(y, ch), m = w ? unpack8(static_cast<const uint4*>(w)[ch]) : fill8(1.f);
-    const V8 g = p.a.gate && p.a.gate_col_stride ? gate8(p, row, ch) : fill8(g_row);
+    const V8 n = load8<Y>(y, ch);
+    if (g_row == 0.f || !both_nonzero(n, n)) return false;
+    const V8 m = w ? unpack8(static_cast<const uint4*>(w)[ch]) : fill8(1.f);
+    const V8 g = p.a.gate && p.a.gate_col_stride ? gate8(p, row, ch) : fill8(1.f);
     bool any = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i) any |= n.at(i) != 0.f && m.at(i) != 0.f && g.at(i) != 0.f;
@@ -394,6 +392,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                 f = __frsqrt_rn(m);
             }
             const float2 fg = make_float2(f * g_row.x, f * g_row.y), scale = make_float2(a.scale, a.scale);
+            wild |= fabsf(fg.x) < 0x1p-126f && g_row.x != 0.f;
             ss = 0.f;
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
@@ -458,7 +457,7 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
             auto lost_zeros = [&](int c, int ch, float wm, const V8& w) {        // chunk c, of a block of zeros
                 if constexpr (!HAS_Y) return ch < chunks && both_nonzero(load8<R>(sr, ch), w);
                 else if (top[c] > 0.f) return wm > 0.f;
-                else return fmaxf(f, 1.f) * wm > kZeroFactors && lost_product<Y>(p, row, ch, g_row.x, sy, a.post_weight);
+                else return wm > 0.f && lost_product<Y>(p, row, ch, g_row.x, sy, a.post_weight);
             };
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
@@ -738,7 +737,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
     constexpr float kE = 0x1.4p-21f;                                // 10 u
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[kRowWarps];
-    __shared__ uint32_t red_max[kRowWarps];
+    __shared__ uint32_t red_max[kRowWarps], red_post[kRowWarps];
     __shared__ int taken, timeout;
     const nvfp4b_block_norm_args& a = p.a;
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, warps = blockDim.x >> 5, chunks = a.H >> 3;
@@ -771,19 +770,36 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
         if (first < a.T) fetch(first);
     }
     const uint4 ones = make_uint4(0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u);
-    uint32_t wm_bits = 0;
-    for (int ch = threadIdx.x; ch < chunks; ch += blockDim.x) {
-        if (HAS_Y) w_post[ch] = a.post_weight ? static_cast<const uint4*>(a.post_weight)[ch] : ones;
-        const uint4 q = a.norm_weight ? static_cast<const uint4*>(a.norm_weight)[ch] : ones;
-        w_norm[ch] = q;
+    auto top8 = [](const uint4& q) {                                // largest magnitude of eight bf16
         const uint32_t m = __vmaxu2(__vmaxu2(q.x & 0x7FFF7FFFu, q.y & 0x7FFF7FFFu),
                                     __vmaxu2(q.z & 0x7FFF7FFFu, q.w & 0x7FFF7FFFu));
-        wm_bits = max(wm_bits, max(m & 0xFFFFu, m >> 16));
+        return max(m & 0xFFFFu, m >> 16);
+    };
+    uint32_t wm_bits = 0, post_bits = 0;
+    for (int ch = threadIdx.x; ch < chunks; ch += blockDim.x) {
+        const uint4 q = a.norm_weight ? __ldg(static_cast<const uint4*>(a.norm_weight) + ch) : ones;
+        if constexpr (HAS_Y) {
+            const uint4 q1 = a.post_weight ? __ldg(static_cast<const uint4*>(a.post_weight) + ch) : ones;
+            w_post[ch] = q1;
+            post_bits = max(post_bits, top8(q1));
+        }
+        w_norm[ch] = q;
+        wm_bits = max(wm_bits, top8(q));
     }
     wm_bits = __reduce_max_sync(0xFFFFFFFFu, wm_bits);
-    if (lane == 0) red_max[wid] = wm_bits;
+    post_bits = __reduce_max_sync(0xFFFFFFFFu, post_bits);
+    if (lane == 0) {
+        red_max[wid] = wm_bits;
+        red_post[wid] = post_bits;
+    }
     __syncthreads();
     const float wm = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, lane < warps ? red_max[lane] : 0u) << 16);
+    // Blocks of zeros: true ones, or products that underflowed.  Such a product is below 2^-149, so it matters (the least border
+    // is 2^-129) only where the factors behind it make more than 2^18: the weights, 1 / rms(r), a gate per feature.  Below, a code
+    // of 0 may have the sign of the rounded product and not of the product: looking at every block of zeros took 10% more where
+    // half the rows are.
+    const uint32_t post_max = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? red_post[lane] : 0u) << 16;
+    const float factors = HAS_Y && a.gate && a.gate_col_stride ? __int_as_float(0x7F800000) : wm * fmaxf(__uint_as_float(post_max), 1.f);
     __syncthreads();                                                // red_max is used again at the end
 
     uint32_t zmax = 0, phase = 0;
@@ -812,6 +828,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
                 f = __frsqrt_rn(m);
             }
             fgs = f * g_row * a.scale;
+            wild |= fabsf(fgs) < 0x1p-126f && g_row != 0.f && a.scale != 0.f;
         }
         const float2 scale2 = make_float2(a.scale, a.scale);
         float t_max = 0.f, st = 0.f;
@@ -947,7 +964,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
             }
         }
         if constexpr (MX) {
-            if (fmaxf(f, 1.f) * wm <= kZeroFactors) {
+            if (fmaxf(f, 1.f) * factors <= 0x1p18f) {
                 doubt &= ~zeros;
             } else {
                 for (; zeros; zeros &= zeros - 1) {

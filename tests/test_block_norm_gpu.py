@@ -454,3 +454,42 @@ def test_rows_of_one_element(T, H, dtype):
         ref = mx.quantize(_n(z))
         byte, _ = mx.untile_scales(got.scales.cpu().numpy(), T, H)
         assert np.array_equal(byte, ref[1]) and np.array_equal(got.codes.cpu().numpy(), ref[0])
+
+
+@pytest.mark.parametrize("T", [12, 1300])
+@pytest.mark.parametrize("resid", [None, F])
+@pytest.mark.parametrize("dtype", [B, F])
+def test_gate_over_rms_that_underflows(T, resid, dtype):
+    """gate / rms(y) below fp32 while gate * n is not."""
+    p = require_gpu()
+    for g_exp, scale in [(-110, 1.0), (-85, 1.0), (-85, 2.0 ** -30), (-60, 2.0 ** -60)]:
+        kw = _make(T, 256, 25, resid, dtype, gate="row")
+        kw["y"] *= 2.0 ** 45
+        kw["gate"] *= 2.0 ** g_exp
+        if resid:
+            kw["resid"][:, 32:96], kw["resid"][::2] = 0.0, 0.0
+        for mx_too, out_too in [(True, False), (True, True), (False, True)]:
+            _check(p, T, 256, mx_too, out_too, scale=scale, **kw)
+
+
+@pytest.mark.parametrize("T", [12, 1300])
+@pytest.mark.parametrize("resid", [None, F])
+def test_inputs_that_underflow_before_the_weight(T, resid):
+    """y / rms(y) below fp32 where the post weight or a gate brings it back: the codes."""
+    p = require_gpu()
+    H = 256
+    for gate, w_exp, g_exp in [("", 40, 0), ("row", 40, 0), ("feature", 20, 20), ("full", 20, 20), ("feature", 0, 40)]:
+        kw = _make(T, H, 26, resid, B, gate=gate)
+        kw["y"] *= 2.0 ** 30
+        kw["y"][:, 32:64] *= 2.0 ** -100
+        kw["y"][:, 32:64] *= 2.0 ** -55                            # 2^-125, and 2^-155 after the norm
+        kw["post_weight"][32:64] *= 2.0 ** w_exp
+        if g_exp:
+            kw["gate"][..., 32:64] *= 2.0 ** g_exp
+        if resid:
+            kw["resid"][:, 32:64] = 0.0
+        codes, scales = poisoned(T * H // 2).view(T, H // 2), poisoned(mx.scale_buffer_bytes(T, H))
+        p.block_norm(codes=codes, scales=scales, **kw)
+        ref = mx.quantize(_want(kw)[1])
+        byte, clean = mx.untile_scales(scales.cpu().numpy(), T, H)
+        assert np.array_equal(byte, ref[1]) and clean and np.array_equal(codes.cpu().numpy(), ref[0])
