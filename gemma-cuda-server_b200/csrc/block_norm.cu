@@ -495,7 +495,8 @@ __global__ void __launch_bounds__(kNormMaxThreads, 1) block_norm_kernel(const __
                     }
                     code[c] = cvt_e2m1x8(lo[0].x, lo[0].y, lo[1].x, lo[1].y, lo[2].x, lo[2].y, lo[3].x, lo[3].y);
                     const uint32_t up = cvt_e2m1x8(hi[0].x, hi[0].y, hi[1].x, hi[1].y, hi[2].x, hi[2].y, hi[3].x, hi[3].y);
-                    const bool doubt = ((code[c] ^ up) & kCodeBits<HAS_Y>) != 0u || byte[c] != mx_byte(__float_as_uint(fmaxf(zm - dm, 0.f))) ||
+                    const bool doubt = ((code[c] ^ up) & kCodeBits<HAS_Y>) != 0u ||
+                                       byte[c] != mx_byte(__float_as_uint(fmaxf(zm - dm, 0.f))) ||
                                        top_bits >= 0x7F000000u ||
                                        (top_bits < 0x21800000u &&                      // below 2^-60, or lost
                                         (top_bits != 0u || lost_zeros(c, ch, wm, w))) ||
@@ -799,7 +800,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 1) block_norm_rows_kernel(cons
     // of 0 may have the sign of the rounded product and not of the product: looking at every block of zeros took 10% more where
     // half the rows are.
     const uint32_t post_max = __reduce_max_sync(0xFFFFFFFFu, lane < warps ? red_post[lane] : 0u) << 16;
-    const float factors = HAS_Y && a.gate && a.gate_col_stride ? __int_as_float(0x7F800000) : wm * fmaxf(__uint_as_float(post_max), 1.f);
+    const float factors =
+        HAS_Y && a.gate && a.gate_col_stride ? __int_as_float(0x7F800000) : wm * fmaxf(__uint_as_float(post_max), 1.f);
     __syncthreads();                                                // red_max is used again at the end
 
     uint32_t zmax = 0, phase = 0;
@@ -1145,7 +1147,9 @@ bool clash(const Region& a, const Region& b, bool same = false) {
 
 // Whether an output shares memory with another one, or with an input (resid_out and out may be resid or y themselves).
 bool clashes(const nvfp4b_block_norm_args& a) {
-    const auto rows = [&](const void* p, int f32, long long ld) { return Region(p, a.H * (f32 ? 4ll : 2ll), ld * (f32 ? 4 : 2), a.T); };
+    const auto rows = [&](const void* p, int f32, long long ld) {
+        return Region(p, a.H * (f32 ? 4ll : 2ll), ld * (f32 ? 4 : 2), a.T);
+    };
     const long long gate_size = a.gate_f32 ? 4 : 2;
     const Region out[] = {rows(a.resid_out, a.resid_out_f32, a.ld_resid_out), rows(a.out, 0, a.ld_out),
                           Region(a.codes, (long long)a.T * (a.H / 2)),
